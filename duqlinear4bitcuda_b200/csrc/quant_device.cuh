@@ -53,9 +53,9 @@ __device__ __forceinline__ RowQ load_rowq(const __half *s1, const __half *z1, co
 // not HBM-bound). Valid for a row whose scales are finite and non-zero, whose zero-points are
 // finite (|rint(z)| <= 400 for the single-scale asymmetric scheme) and which contains no
 // inf/NaN -- everything else takes code8<MODE>.
-//   * __hdiv(x, s) is half(rcp.approx.ftz(float(s)) * float(x)) plus a refinement that only
-//     fires for quotients below 8.6e-6, which round to the same code either way; the reciprocal
-//     is taken once per row with the same instruction.
+//   * the quotient is the scale's approximate reciprocal (PTX rcp.approx.ftz.f32, taken once per row) times x in fp32,
+//     rounded once to fp16; that its codes equal those of the element-by-element division is what
+//     tests/test_gpu_quant_fused_vs_reference_kernel.py requires, byte for byte.
 //   * rounding to integer and clamping happen in fp16x2: adding 1024 + offset to a value already
 //     clamped to a 16-wide integer window rounds it to nearest-even exactly like
 //     __half2int_rn, and leaves the code in the low four bits of each half.

@@ -42,10 +42,9 @@ static inline float nudge_f32(float f, int n) {
     return f;
 }
 
-/* __hdiv. Host branch of the CUDA header: half(float(a)/float(b)). The device branch is
- * rcp.approx(b)*a, within ~2 ulp(fp32) of the exact quotient; `nudge` moves the fp32
- * quotient by that many ulps away from (+) or toward (-) zero so a caller can bracket
- * it. (include/cuda_fp16.hpp, __hdiv.) */
+/* Half division: half(float(a)/float(b)). The GPU's quotient may differ from the exact one in its last fp32
+ * places; `nudge` moves the fp32 quotient by that many ulps away from (+) or toward (-) zero so a caller can
+ * bracket it. */
 static inline h16 hdiv_n(h16 a, h16 b, int nudge) {
     float q = h2f(a) / h2f(b);
     return f2h(nudge_f32(q, nudge));
