@@ -579,6 +579,201 @@ Tensor linear_w4a4_batched(const std::string &mode, const Tensor &A, const Tenso
     return out;
 }
 
+// ---- microscaled 4-bit floating point (new) -------------------------------------------------------------------
+int fp4_format_of(const char *fn, const std::string &f) {
+    if (f == "mxfp4") return DUQ4_FP4_MX;
+    if (f == "nvfp4") return DUQ4_FP4_NV;
+    TORCH_CHECK(false, fn, ": unknown format '", f, "' (mxfp4, nvfp4)");
+    return 0;
+}
+int dtype16_of(const char *fn, torch::ScalarType t, const char *name) {
+    if (t == torch::kFloat16) return DUQ4_DTYPE_F16;
+    if (t == torch::kBFloat16) return DUQ4_DTYPE_BF16;
+    TORCH_CHECK(false, fn, ": expected ", name, " to have dtype Half or BFloat16, got ", c10::toString(t));
+    return 0;
+}
+// Sizes go to the library as 32-bit numbers.
+uint32_t size32(const char *fn, const Tensor &t, int64_t dim, const char *name) {
+    TORCH_CHECK(t.size(dim) <= 0x7FFFFFFF, fn, ": ", name, " is too large");
+    return (uint32_t)t.size(dim);
+}
+struct Fp4Out {
+    Tensor codes, block_scales, row_scales;   // row_scales undefined for mxfp4
+    float *rows() const { return row_scales.defined() ? row_scales.data_ptr<float>() : nullptr; }
+    py::object row_object() const { return row_scales.defined() ? py::cast(row_scales) : py::none(); }
+    py::tuple tuple() const { return py::make_tuple(codes, block_scales, row_object()); }
+};
+void check_fp4_cols(const char *fn, int64_t cols, const char *name) {
+    TORCH_CHECK(cols > 0 && cols % 32 == 0, fn, ": expected ", name, " to be a positive multiple of 32, got ", cols);
+}
+Fp4Out fp4_out(const Tensor &ref, int format, uint32_t rows, uint32_t cols) {
+    Fp4Out o;
+    o.codes = empty_like_dev(ref, {rows, cols / 2}, torch::kUInt8);
+    o.block_scales = empty_like_dev(ref, {(int64_t)duq4_fp4_scale_bytes(format, rows, cols)}, torch::kUInt8);
+    if (format == DUQ4_FP4_NV) o.row_scales = empty_like_dev(ref, {rows}, torch::kFloat32);
+    return o;
+}
+
+// (new) x fp16 / bfloat16 [rows, K] -> (codes uint8 [rows, K/2], block scales uint8 in the tensor cores' tile order, row
+// scales float [rows] or None). format: "mxfp4" or "nvfp4"; see duq4_fp4_quantize.
+py::tuple fp4_quantize(const std::string &format, const Tensor &x) {
+    const char *fn = "fp4_quantize";
+    const int f = fp4_format_of(fn, format), dt = dtype16_of(fn, x.scalar_type(), "x");
+    TORCH_CHECK(x.dim() == 2, fn, ": expected x to be 2-D");
+    check_tensors(fn, {{&x, "x"}});
+    check_fp4_cols(fn, x.size(1), "x.size(1)");
+    const uint32_t rows = size32(fn, x, 0, "x"), cols = size32(fn, x, 1, "x");
+    Launch l(x);
+    const Fp4Out o = fp4_out(x, f, rows, cols);
+    ok(fn, duq4_fp4_quantize(f, dt, x.data_ptr(), rows, cols, cols, o.codes.data_ptr<uint8_t>(), o.block_scales.data_ptr<uint8_t>(), o.rows(), l.stream));
+    return o.tuple();
+}
+
+// (new) gate_up fp16 / bfloat16 [rows, 2*I], gate projection in columns [0, I), up projection in [I, 2I): the quantized
+// form of F.silu(gate) * up, which is not stored.
+py::tuple fp4_silu_mul_quantize(const std::string &format, const Tensor &gate_up) {
+    const char *fn = "fp4_silu_mul_quantize";
+    const int f = fp4_format_of(fn, format), dt = dtype16_of(fn, gate_up.scalar_type(), "gate_up");
+    TORCH_CHECK(gate_up.dim() == 2 && gate_up.size(1) % 2 == 0, fn, ": expected gate_up to be [rows, 2*I]");
+    check_tensors(fn, {{&gate_up, "gate_up"}});
+    check_fp4_cols(fn, gate_up.size(1) / 2, "I");
+    const uint32_t rows = size32(fn, gate_up, 0, "gate_up"), ld = size32(fn, gate_up, 1, "gate_up"), inter = ld / 2;
+    Launch l(gate_up);
+    const Fp4Out o = fp4_out(gate_up, f, rows, inter);
+    ok(fn, duq4_fp4_silu_mul_quantize(f, dt, gate_up.data_ptr(), rows, inter, ld, inter, o.codes.data_ptr<uint8_t>(),
+                                      o.block_scales.data_ptr<uint8_t>(), o.rows(), l.stream));
+    return o.tuple();
+}
+
+// A quantized tensor handed back: codes [rows, K/2], block scales of the size the format needs, row scales [rows] (optional
+// = 1 in the product, required for reading nvfp4 back).
+void check_fp4_operand(const char *fn, int format, const Tensor &codes, const char *codes_name, const Tensor &scales, const char *scales_name,
+                       const OptTensor &rows, const char *rows_name) {
+    TORCH_CHECK(codes.dim() == 2, fn, ": expected ", codes_name, " to be 2-D");
+    check_fp4_cols(fn, codes.size(1) * 2, "K");
+    const int64_t need = (int64_t)duq4_fp4_scale_bytes(format, size32(fn, codes, 0, codes_name), size32(fn, codes, 1, codes_name) * 2);
+    TORCH_CHECK(scales.numel() == need, fn, ": expected ", scales_name, " to have ", need, " bytes, got ", scales.numel());
+    if (opt(rows)) TORCH_CHECK(rows->numel() == codes.size(0), fn, ": expected ", rows_name, " to have ", codes.size(0), " entries, got ", rows->numel());
+}
+
+// (new) the values of a quantized tensor [rows, K], rounded once to dtype (fp16, bfloat16 or float32).
+Tensor fp4_dequantize(const std::string &format, const Tensor &codes, const Tensor &block_scales, const OptTensor &row_scales, torch::ScalarType dtype) {
+    const char *fn = "fp4_dequantize";
+    const int f = fp4_format_of(fn, format), dt = dtype == torch::kFloat32 ? DUQ4_DTYPE_F32 : dtype16_of(fn, dtype, "the result");
+    check_tensors(fn, {{&codes, "codes", torch::kUInt8}, {&block_scales, "block_scales", torch::kUInt8}, {opt(row_scales), "row_scales", torch::kFloat32}});
+    check_fp4_operand(fn, f, codes, "codes", block_scales, "block_scales", row_scales, "row_scales");
+    TORCH_CHECK((f == DUQ4_FP4_NV) == (opt(row_scales) != nullptr), fn, ": row_scales go with nvfp4 and only with it");
+    const uint32_t rows = codes.size(0), cols = codes.size(1) * 2;
+    Launch l(codes);
+    auto out = empty_like_dev(codes, {rows, cols}, dtype);
+    ok(fn, duq4_fp4_dequantize(f, dt, codes.data_ptr<uint8_t>(), block_scales.data_ptr<uint8_t>(), (const float *)ptr(row_scales), rows, cols, out.data_ptr(),
+                               l.stream));
+    return out;
+}
+
+// (new) The joint between two blocks (see duq4_norm_residual_quantize): with `residual`, the stream becomes
+// residual + residual_scale * gate * [norm(x) * post_weight], else it is x; its norm times `weight` is returned quantized.
+// format: "none" -> (stream, h), "sym" -> (stream, codes, scales), "asym" -> (stream, codes, scales, zeros), "mxfp4" /
+// "nvfp4" -> (stream, codes, block_scales, row_scales). The stream is None without residual. gate: [C] or [rows, C].
+py::tuple norm_residual_quantize(const std::string &format, const Tensor &x, const Tensor &weight, double eps, const OptTensor &residual,
+                                 const OptTensor &post_weight, const OptTensor &gate, double residual_scale, double clip_ratio) {
+    const char *fn = "norm_residual_quantize";
+    const int f = format == "none" ? DUQ4_MODE_NONE : format == "sym" ? DUQ4_MODE_SYM : format == "asym" ? DUQ4_MODE_ASYM : fp4_format_of(fn, format);
+    const auto st = x.scalar_type();
+    duq4_norm_residual n = {};
+    n.dtype = dtype16_of(fn, st, "x");
+    TORCH_CHECK(n.dtype == DUQ4_DTYPE_F16 || (f != DUQ4_MODE_SYM && f != DUQ4_MODE_ASYM), fn, ": sym and asym take Half tensors");
+    check_tensors(fn, {{&x, "x"}, {&weight, "weight", st}, {opt(residual), "residual", st}, {opt(post_weight), "post_weight", st}, {opt(gate), "gate", st}});
+    TORCH_CHECK(x.dim() == 2, fn, ": expected x to be 2-D");
+    const uint32_t rows = size32(fn, x, 0, "x"), cols = size32(fn, x, 1, "x");
+    check_fp4_cols(fn, cols, "x.size(1)");
+    TORCH_CHECK(weight.numel() == cols, fn, ": expected weight to have ", cols, " entries, got ", weight.numel());
+    TORCH_CHECK(opt(residual) || (!opt(post_weight) && !opt(gate)), fn, ": post_weight and gate go with residual");
+    TORCH_CHECK(eps >= 0, fn, ": eps must not be negative");
+    Tensor stream_out;
+    Launch l(x);
+    if (opt(residual)) {
+        TORCH_CHECK(residual->sizes() == x.sizes(), fn, ": residual and x disagree on their shape");
+        if (opt(post_weight)) TORCH_CHECK(post_weight->numel() == cols, fn, ": expected post_weight to have ", cols, " entries, got ", post_weight->numel());
+        if (opt(gate)) {
+            TORCH_CHECK(gate->sizes() == x.sizes() || (gate->dim() == 1 && gate->size(0) == cols), fn, ": gate must be [C] or [rows, C]");
+            n.gate_per_row = gate->dim() == 2;
+        }
+        stream_out = empty_like_dev(x, {rows, cols}, st);
+        n.residual = residual->data_ptr();
+        n.residual_out = stream_out.data_ptr();
+    }
+    n.eps = eps;
+    n.residual_scale = (float)residual_scale;
+    n.clip_ratio = (float)clip_ratio;
+    n.x = x.data_ptr();
+    n.weight = weight.data_ptr();
+    n.post_weight = ptr(post_weight);
+    n.gate = ptr(gate);
+    const py::object stream_object = stream_out.defined() ? py::cast(stream_out) : py::none();
+    if (f == DUQ4_FP4_MX || f == DUQ4_FP4_NV) {
+        const Fp4Out o = fp4_out(x, f, rows, cols);
+        ok(fn, duq4_norm_residual_quantize(f, &n, rows, cols, o.codes.data_ptr(), o.block_scales.data_ptr(), o.rows(), l.stream));
+        return py::make_tuple(stream_object, o.codes, o.block_scales, o.row_object());
+    }
+    if (f == DUQ4_MODE_NONE) {
+        auto h = empty_like_dev(x, {rows, cols}, st);
+        ok(fn, duq4_norm_residual_quantize(f, &n, rows, cols, h.data_ptr(), nullptr, nullptr, l.stream));
+        return py::make_tuple(stream_object, h);
+    }
+    auto q = empty_like_dev(x, {rows, cols / 2}, torch::kUInt8);
+    auto s = row_vec(x, rows);
+    Tensor z;
+    if (f == DUQ4_MODE_ASYM) z = row_vec(x, rows);
+    ok(fn, duq4_norm_residual_quantize(f, &n, rows, cols, q.data_ptr(), s.data_ptr(), z.defined() ? z.data_ptr() : nullptr, l.stream));
+    if (z.defined()) return py::make_tuple(stream_object, q, s, z);
+    return py::make_tuple(stream_object, q, s);
+}
+
+// (new) [M, N] of `dtype` (None = fp16) = A [M, K] x W [N, K]^T of two quantized tensors of one format, times the per-token and
+// per-channel factors (None = 1), plus bias.
+Tensor linear_fp4(const std::string &format, const Tensor &A, const Tensor &A_block_scales, const OptTensor &A_row_scales, const Tensor &W,
+                  const Tensor &W_block_scales, const OptTensor &W_row_scales, const OptTensor &bias, std::optional<torch::ScalarType> dtype_) {
+    const char *fn = "linear_fp4";
+    const torch::ScalarType dtype = dtype_.value_or(torch::kFloat16);
+    constexpr auto U8 = torch::kUInt8, F32 = torch::kFloat32;
+    const int f = fp4_format_of(fn, format), dt = dtype16_of(fn, dtype, "the result");
+    check_tensors(fn, {{&A, "A", U8}, {&A_block_scales, "A_block_scales", U8}, {opt(A_row_scales), "A_row_scales", F32}, {&W, "W", U8},
+                       {&W_block_scales, "W_block_scales", U8}, {opt(W_row_scales), "W_row_scales", F32}, {opt(bias), "bias", dtype}});
+    check_fp4_operand(fn, f, A, "A", A_block_scales, "A_block_scales", A_row_scales, "A_row_scales");
+    check_fp4_operand(fn, f, W, "W", W_block_scales, "W_block_scales", W_row_scales, "W_row_scales");
+    TORCH_CHECK(A.size(1) == W.size(1), fn, ": A and W disagree on K");
+    const uint32_t M = A.size(0), N = W.size(0), K = A.size(1) * 2;
+    if (opt(bias)) TORCH_CHECK(bias->numel() == (int64_t)N, fn, ": expected bias to have ", N, " entries, got ", bias->numel());
+    Launch l(A);
+    auto out = empty_like_dev(A, {M, N}, dtype);
+    ok(fn, duq4_linear_fp4(f, A.data_ptr<uint8_t>(), A_block_scales.data_ptr<uint8_t>(), (const float *)ptr(A_row_scales), W.data_ptr<uint8_t>(),
+                           W_block_scales.data_ptr<uint8_t>(), (const float *)ptr(W_row_scales), M, N, K, ptr(bias), dt, out.data_ptr(), N, l.stream));
+    return out;
+}
+
+// (new) the same from 16-bit activations x [M, K], quantized per token on the way; the result has x's type. The quantized
+// tokens live in a tensor of this call, so that calls on other streams and captured graphs have their own.
+Tensor linear_fp4_from_16bit(const std::string &format, const Tensor &x, const Tensor &W, const Tensor &W_block_scales, const OptTensor &W_row_scales,
+                             const OptTensor &bias) {
+    const char *fn = "linear_fp4_from_16bit";
+    const auto st = x.scalar_type();
+    const int f = fp4_format_of(fn, format), dt = dtype16_of(fn, st, "x");
+    check_tensors(fn, {{&x, "x"}, {&W, "W", torch::kUInt8}, {&W_block_scales, "W_block_scales", torch::kUInt8}, {opt(W_row_scales), "W_row_scales", torch::kFloat32},
+                       {opt(bias), "bias", st}});
+    check_fp4_operand(fn, f, W, "W", W_block_scales, "W_block_scales", W_row_scales, "W_row_scales");
+    TORCH_CHECK(x.dim() == 2 && x.size(1) == W.size(1) * 2, fn, ": x and W disagree on K");
+    const uint32_t M = size32(fn, x, 0, "x"), N = W.size(0), K = W.size(1) * 2;
+    if (opt(bias)) TORCH_CHECK(bias->numel() == (int64_t)N, fn, ": expected bias to have ", N, " entries, got ", bias->numel());
+    Launch l(x);
+    auto out = empty_like_dev(x, {M, N}, st);
+    const size_t need = duq4_linear_fp4_workspace_bytes(f, M, K);
+    auto ws = empty_like_dev(x, {(int64_t)need}, torch::kUInt8);
+    ok(fn, duq4_linear_fp4_from_16bit(f, dt, x.data_ptr(), W.data_ptr<uint8_t>(), W_block_scales.data_ptr<uint8_t>(), (const float *)ptr(W_row_scales), M, N, K,
+                                      ptr(bias), out.data_ptr(), N, ws.data_ptr(), need, l.stream));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -624,4 +819,14 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("linear_w4a4_batched", &linear_w4a4_batched, py::arg("mode"), py::arg("A"), py::arg("W"), py::arg("scale_row"),
           py::arg("zeros_row") = py::none(), py::arg("scale_col_1") = py::none(), py::arg("zeros_col_1") = py::none(),
           py::arg("scale_col_2") = py::none(), py::arg("zeros_col_2") = py::none());
+    m.def("fp4_quantize", &fp4_quantize, py::arg("format"), py::arg("x"));
+    m.def("fp4_silu_mul_quantize", &fp4_silu_mul_quantize, py::arg("format"), py::arg("gate_up"));
+    m.def("fp4_dequantize", &fp4_dequantize, py::arg("format"), py::arg("codes"), py::arg("block_scales"), py::arg("row_scales"), py::arg("dtype"));
+    m.def("norm_residual_quantize", &norm_residual_quantize, py::arg("format"), py::arg("x"), py::arg("weight"), py::arg("eps") = 1e-6,
+          py::arg("residual") = py::none(), py::arg("post_weight") = py::none(), py::arg("gate") = py::none(), py::arg("residual_scale") = 1.0,
+          py::arg("clip_ratio") = 1.0);
+    m.def("linear_fp4", &linear_fp4, py::arg("format"), py::arg("A"), py::arg("A_block_scales"), py::arg("A_row_scales"), py::arg("W"),
+          py::arg("W_block_scales"), py::arg("W_row_scales"), py::arg("bias") = py::none(), py::arg("dtype") = py::none());
+    m.def("linear_fp4_from_16bit", &linear_fp4_from_16bit, py::arg("format"), py::arg("x"), py::arg("W"), py::arg("W_block_scales"),
+          py::arg("W_row_scales"), py::arg("bias") = py::none());
 }

@@ -1,0 +1,489 @@
+// Quantizers of the microscaled 4-bit formats and the operators that end in one: activations as they are, the SiLU-gated
+// product of a gate/up projection, and the residual sum between two blocks with its norms. One row kernel does all three:
+// a row is formed in registers, 16 neighbours per thread, and coded from there, so that no intermediate goes to memory.
+// No counterpart in the reference, whose quantizers are integer ones (qlinear4bit/nn/quantizer.py).
+#include "fp4_common.cuh"
+#include "quant_device.cuh"
+#include "trace_range.h"
+
+namespace duq4 {
+namespace fp4 {
+
+enum { SRC_PLAIN, SRC_SILU, SRC_NORM };
+enum { OUT_ROW = DUQ4_MODE_NONE, OUT_SYM = DUQ4_MODE_SYM, OUT_ASYM = DUQ4_MODE_ASYM, OUT_MX = kMX, OUT_NV = kNV };
+
+struct RowArgs {
+    uint32_t rows, cols;
+    uint64_t ldx;                 // elements between rows of x
+    const uint16_t *x;            // SRC_SILU: gate and up projections side by side
+    uint32_t up_offset;
+    // SRC_NORM
+    const uint16_t *residual, *post_weight, *gate, *weight;
+    uint16_t *residual_out;
+    uint32_t gate_per_row;
+    float residual_scale;
+    double eps;
+    float clip;
+    // results
+    uint8_t *codes;               // OUT_ROW: the 16-bit row itself
+    uint8_t *block_scales;        // OUT_SYM / OUT_ASYM: fp16 scales [rows]
+    void *row_scales;             // OUT_NV: float [rows]; OUT_ASYM: fp16 zero-points [rows]
+};
+
+struct Chunk {                    // 16 neighbours of a row
+    uint32_t w[8];
+};
+__device__ __forceinline__ Chunk load_chunk(const uint16_t *p) {
+    Chunk c;
+    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p)), b = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
+    c.w[0] = a.x; c.w[1] = a.y; c.w[2] = a.z; c.w[3] = a.w;
+    c.w[4] = b.x; c.w[5] = b.y; c.w[6] = b.z; c.w[7] = b.w;
+    return c;
+}
+// The same without the read-only path, for tensors that the call may write in place.
+__device__ __forceinline__ Chunk load_chunk_rw(const uint16_t *p) {
+    Chunk c;
+    const uint4 a = reinterpret_cast<const uint4 *>(p)[0], b = reinterpret_cast<const uint4 *>(p)[1];
+    c.w[0] = a.x; c.w[1] = a.y; c.w[2] = a.z; c.w[3] = a.w;
+    c.w[4] = b.x; c.w[5] = b.y; c.w[6] = b.z; c.w[7] = b.w;
+    return c;
+}
+__device__ __forceinline__ void store_chunk(uint16_t *p, const Chunk &c) {
+    reinterpret_cast<uint4 *>(p)[0] = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]);
+    reinterpret_cast<uint4 *>(p)[1] = make_uint4(c.w[4], c.w[5], c.w[6], c.w[7]);
+}
+
+// h = silu(g) * u with the roundings of F.silu(gate) * up on 16-bit tensors: silu in 32 bits, rounded, then the product.
+template <class T>
+__device__ __forceinline__ uint32_t silu_mul_two(uint32_t g, uint32_t u) {
+    const float2 x = Two<T>::up(g), y = Two<T>::up(u);
+    const float2 s = Two<T>::up(Two<T>::down(__fdiv_rn(x.x, 1.0f + expf(-x.x)), __fdiv_rn(x.y, 1.0f + expf(-x.y))));
+    return Two<T>::down(__fmul_rn(s.x, y.x), __fmul_rn(s.y, y.y));
+}
+
+// Sums over the block; every thread gets the result. `sm` must not be in use by an earlier reduction's readers.
+template <int NT>
+__device__ __forceinline__ double block_sum(double v, double *sm) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double r = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) r += sm[w];
+    return r;
+}
+template <int NT>
+__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *sm) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+    __syncthreads();
+    uint32_t r = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) r = max(r, sm[w]);
+    return r;
+}
+
+// 1 / sqrt(mean of squares + eps) of the row that the block's threads hold. Codes jump at borders and the layer behind
+// must not depend on the order of a sum, so the sum is carried with its rounding errors: squares of 16-bit values are
+// exact in 32 bits, and each addition's error is recovered (Knuth's two-sum) and summed beside. Only rows whose
+// squares leave the range of 32 bits (bfloat16 beyond 1e19, infinities) are summed again in 64 bits.
+template <class T, int NT, int CH>
+__device__ __forceinline__ float row_rstd(const Chunk (&d)[CH], uint32_t chunks, uint32_t cols, double eps, double *sm) {
+    float s = 0.f, c = 0.f;
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+        if (threadIdx.x + i * NT < chunks) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float2 x = Two<T>::up(d[i].w[k]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float p = __fmul_rn(h ? x.y : x.x, h ? x.y : x.x);
+                    const float t = __fadd_rn(s, p), b = __fsub_rn(t, s);
+                    c = __fadd_rn(c, __fadd_rn(__fsub_rn(s, __fsub_rn(t, b)), __fsub_rn(p, b)));
+                    s = t;
+                }
+            }
+        }
+    double sum = block_sum<NT>((double)s + (double)c, sm);
+    if (!(sum > 1e-24 && sum < 1e38)) {   // the same for every thread
+        double v = 0;
+#pragma unroll
+        for (int i = 0; i < CH; ++i)
+            if (threadIdx.x + i * NT < chunks) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float2 x = Two<T>::up(d[i].w[k]);
+                    v += (double)x.x * x.x + (double)x.y * x.y;
+                }
+            }
+        __syncthreads();
+        sum = block_sum<NT>(v, sm);
+    }
+    return (float)(1.0 / sqrt(sum / cols + eps));
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t chunk_top(const Chunk &c) {   // largest magnitude's bits (above kInf: a NaN)
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) m = __vmaxu2(m, c.w[k] & 0x7FFF7FFFu);
+    return max(m & 0xFFFFu, m >> 16);
+}
+
+// One CTA of NT threads per row, CH chunks per thread.
+template <int SRC, class T, int OUT, int NT, int CH>
+__global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
+    __shared__ double sm_d[2][NT / 32];
+    __shared__ uint32_t sm_u[NT / 32];
+    __shared__ float sm_f[NT / 32][4];
+    const uint32_t chunks = a.cols >> 4;
+    const int lane = threadIdx.x & 31;
+    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        Chunk d[CH];
+        const uint16_t *xr = a.x + (size_t)row * a.ldx;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const uint32_t c = threadIdx.x + i * NT;
+            if (c < chunks) {
+                d[i] = SRC == SRC_NORM ? load_chunk_rw(xr + c * 16) : load_chunk(xr + c * 16);
+                if (SRC == SRC_SILU) {
+                    const Chunk u = load_chunk(xr + a.up_offset + c * 16);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) d[i].w[k] = silu_mul_two<T>(d[i].w[k], u.w[k]);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) d[i].w[k] = 0;
+            }
+        }
+        if (SRC == SRC_NORM) {
+            const size_t base = (size_t)row * a.cols;
+            if (a.residual) {
+                float rstd = 1.f;
+                if (a.post_weight) rstd = row_rstd<T, NT, CH>(d, chunks, a.cols, a.eps, sm_d[0]);
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const uint32_t c = threadIdx.x + i * NT;
+                    if (c >= chunks) continue;
+                    const Chunk r = load_chunk_rw(a.residual + base + c * 16);
+                    Chunk pw, g;
+                    if (a.post_weight) pw = load_chunk(a.post_weight + c * 16);
+                    if (a.gate) g = load_chunk(a.gate + (a.gate_per_row ? base : 0) + c * 16);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        float2 y = Two<T>::up(d[i].w[k]);
+                        const float2 rr = Two<T>::up(r.w[k]);
+                        if (a.post_weight) {
+                            const float2 w = Two<T>::up(pw.w[k]);
+                            y.x = __fmul_rn(__fmul_rn(y.x, rstd), w.x);
+                            y.y = __fmul_rn(__fmul_rn(y.y, rstd), w.y);
+                        }
+                        if (a.gate) {
+                            const float2 w = Two<T>::up(g.w[k]);
+                            y.x = __fmul_rn(y.x, w.x);
+                            y.y = __fmul_rn(y.y, w.y);
+                        }
+                        d[i].w[k] = Two<T>::down(__fadd_rn(rr.x, __fmul_rn(y.x, a.residual_scale)),
+                                                 __fadd_rn(rr.y, __fmul_rn(y.y, a.residual_scale)));
+                    }
+                    store_chunk(a.residual_out + base + c * 16, d[i]);
+                }
+            }
+            const float rstd = row_rstd<T, NT, CH>(d, chunks, a.cols, a.eps, sm_d[1]);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const uint32_t c = threadIdx.x + i * NT;
+                if (c >= chunks) continue;
+                const Chunk w = load_chunk(a.weight + c * 16);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float2 x = Two<T>::up(d[i].w[k]), ww = Two<T>::up(w.w[k]);
+                    d[i].w[k] = Two<T>::down(__fmul_rn(__fmul_rn(x.x, rstd), ww.x), __fmul_rn(__fmul_rn(x.y, rstd), ww.y));
+                }
+            }
+        }
+        if (OUT == OUT_ROW) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const uint32_t c = threadIdx.x + i * NT;
+                if (c < chunks) store_chunk(reinterpret_cast<uint16_t *>(a.codes) + (size_t)row * a.cols + c * 16, d[i]);
+            }
+        } else if (OUT == OUT_SYM || OUT == OUT_ASYM) {
+            // the framework's integer formats: statistics, scale and codes of quant_fused_vec_kernel on the row h
+            constexpr int MODE = OUT == OUT_SYM ? QSYM : QASYM;
+            Stats st;
+            stats_init<MODE>(st);
+            uint32_t am = 0;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                if (threadIdx.x + i * NT >= chunks) continue;
+                am = max(am, chunk_top<T>(d[i]));
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float2 x = Two<T>::up(d[i].w[k]);
+                    stats_add<MODE>(st, x.x, 16);
+                    stats_add<MODE>(st, x.y, 16);
+                }
+            }
+            const bool special = __syncthreads_or(am >= Two<T>::kInf);
+            stats_reduce<MODE>(st, sm_f);
+            const RowQ r = rowq_from_stats<MODE>(st, a.clip);
+            __half *s1 = reinterpret_cast<__half *>(a.block_scales), *z1 = reinterpret_cast<__half *>(a.row_scales);
+            if (threadIdx.x == 0) store_rowq<MODE>(r, row, s1, z1, nullptr, nullptr);
+            const FastQ fq = make_fastq<MODE>(r, special);
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const uint32_t c = threadIdx.x + i * NT;
+                if (c >= chunks) continue;
+                const uint4 lo = make_uint4(d[i].w[0], d[i].w[1], d[i].w[2], d[i].w[3]);
+                const uint4 hi = make_uint4(d[i].w[4], d[i].w[5], d[i].w[6], d[i].w[7]);
+                uint2 q;
+                q.x = fq.ok ? code8_fast<MODE>(lo, fq) : code8<MODE>(lo, 16, r);
+                q.y = fq.ok ? code8_fast<MODE>(hi, fq) : code8<MODE>(hi, 16, r);
+                *reinterpret_cast<uint2 *>(a.codes + (size_t)row * (a.cols >> 1) + c * 8) = q;
+            }
+        } else {
+            constexpr int FMT = OUT == OUT_NV ? kNV : kMX;
+            const uint32_t tiles = scale_tiles(FMT, a.cols);
+            float row_scale = 1.f;
+            if (FMT == kNV) {
+                uint32_t top = 0;   // over the blocks without infinities and NaNs
+#pragma unroll
+                for (int i = 0; i < CH; ++i) {
+                    const uint32_t t = chunk_top<T>(d[i]);
+                    if (t < Two<T>::kInf) top = max(top, t);
+                }
+                top = block_max<NT>(top, sm_u);
+                // 8 bits, so that 6 * row_scale and block scale * row_scale are exact
+                row_scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(Two<T>::up1(top), 2688.f)));
+                row_scale = fmaxf(row_scale, 7.703719777548943e-34f);   // 2^-110
+                if (threadIdx.x == 0) reinterpret_cast<float *>(a.row_scales)[row] = row_scale;
+            }
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const uint32_t c = threadIdx.x + i * NT;
+                uint32_t top = chunk_top<T>(d[i]);
+                if (FMT == kMX) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                const bool special = top >= Two<T>::kInf;
+                uint32_t scale;
+                float q[2][8];
+                if (FMT == kMX) {
+                    // 2^(floor(log2 top) - 2): the exponent field of the float, less 2
+                    const int e = max((int)(__float_as_uint(Two<T>::up1(top)) >> 23) - 2, 0);
+                    const float inv = special ? 0.f : __uint_as_float((uint32_t)(254 - e) << 23);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 x = Two<T>::up(special ? 0u : d[i].w[k]);
+                        q[k >> 2][2 * (k & 3)] = __fmul_rn(x.x, inv);
+                        q[k >> 2][2 * (k & 3) + 1] = __fmul_rn(x.y, inv);
+                    }
+                    scale = special ? 0xFFu : (uint32_t)e;
+                } else {
+                    scale = special ? 0x7Fu : e4m3_of(__fdiv_rn(Two<T>::up1(top), 6.f * row_scale));
+                    const float dd = special ? 0.f : __fmul_rn(e4m3_to_float(scale), row_scale);
+                    const float inv = dd > 0.f ? __fdiv_rn(1.f, dd) : 0.f;
+                    // quotient by the reciprocal, then one step of refinement: a 16-bit value divided by the 12-bit dd is
+                    // the middle of two codes exactly or is at least 2^-15 away from it, so the code is that of x / dd
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float2 x = Two<T>::up(special ? 0u : d[i].w[k]);
+                        const float a0 = __fmul_rn(x.x, inv), a1 = __fmul_rn(x.y, inv);
+                        q[k >> 2][2 * (k & 3)] = __fmaf_rn(-__fmaf_rn(a0, dd, -x.x), inv, a0);   // (-0 stays -0)
+                        q[k >> 2][2 * (k & 3) + 1] = __fmaf_rn(-__fmaf_rn(a1, dd, -x.y), inv, a1);
+                    }
+                }
+                if (c >= chunks) scale = 0;   // padding blocks of the last scale tile
+                if (c < chunks) {
+                    uint2 w;
+                    w.x = e2m1x8(q[0]);
+                    w.y = e2m1x8(q[1]);
+                    *reinterpret_cast<uint2 *>(a.codes + (size_t)row * (a.cols >> 1) + c * 8) = w;
+                }
+                // four block scales are one word of a tile, stored by the first lane of the 8 (4) that hold them
+                constexpr int kStep = FMT == kMX ? 2 : 1;
+                scale |= __shfl_down_sync(0xffffffffu, scale, kStep) << 8;
+                scale |= __shfl_down_sync(0xffffffffu, scale, 2 * kStep) << 16;
+                if ((lane & (4 * kStep - 1)) == 0 && c < chunks)
+                    *reinterpret_cast<uint32_t *>(a.block_scales + scale_offset(tiles, row, c / (4 * kStep))) = scale;
+            }
+        }
+        __syncthreads();   // the reductions' buffers are free for the next row
+    }
+}
+
+// Codes back to values: code * (block scale * row scale), rounded once. One thread per 16 neighbours.
+template <int FMT, class T>
+__global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
+                                                          const float *__restrict__ row_scales, uint32_t rows, uint32_t cols,
+                                                          T *__restrict__ out) {
+    const uint32_t chunks = cols >> 4, tiles = scale_tiles(FMT, cols);
+    const uint64_t total = (uint64_t)rows * chunks;
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
+        const uint32_t row = (uint32_t)(i / chunks), c = (uint32_t)(i % chunks), blk = FMT == kMX ? c >> 1 : c;
+        float s = block_scale_to_float<FMT>(scales[scale_offset(tiles, row, blk >> 2) + (blk & 3)]);
+        if (FMT == kNV) s = __fmul_rn(s, row_scales[row]);
+        const uint2 w = *reinterpret_cast<const uint2 *>(codes + i * 8);
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float2 f = __half22float2(e2m1x2_to_half2((k < 4 ? w.x : w.y) >> (8 * (k & 3)) & 0xFFu));
+            v[2 * k] = __fmul_rn(f.x, s);
+            v[2 * k + 1] = __fmul_rn(f.y, s);
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                reinterpret_cast<float4 *>(out + i * 16)[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+        } else {
+            Chunk o;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) o.w[k] = Two<T>::down(v[2 * k], v[2 * k + 1]);
+            store_chunk(reinterpret_cast<uint16_t *>(out + i * 16), o);
+        }
+    }
+}
+
+static bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// 16 neighbours per thread and chunk; rows of up to 65536 stay in registers.
+constexpr uint32_t kMaxCols = 65536;
+
+template <int SRC, class T, int OUT>
+static int launch_rows(const RowArgs &a, cudaStream_t st) {
+    const uint32_t chunks = a.cols >> 4;
+    const uint32_t grid = a.rows < 148u * 64u ? a.rows : 148u * 64u;
+    if (chunks <= 128) fp4_row_kernel<SRC, T, OUT, 128, 1><<<grid, 128, 0, st>>>(a);
+    else if (chunks <= 512) fp4_row_kernel<SRC, T, OUT, 256, 2><<<grid, 256, 0, st>>>(a);
+    else if (chunks <= 1024) fp4_row_kernel<SRC, T, OUT, 512, 2><<<grid, 512, 0, st>>>(a);
+    else if (chunks <= 2048) fp4_row_kernel<SRC, T, OUT, 1024, 2><<<grid, 1024, 0, st>>>(a);
+    else fp4_row_kernel<SRC, T, OUT, 1024, 4><<<grid, 1024, 0, st>>>(a);
+    return launch_status();
+}
+
+static int check_fp4(int format, int dtype, uint32_t cols) {
+    if (format != kMX && format != kNV) return DUQ4_ERR_MODE;
+    if (dtype != DUQ4_DTYPE_F16 && dtype != DUQ4_DTYPE_BF16) return DUQ4_ERR_MODE;
+    if (cols == 0 || cols % 32 != 0 || cols > kMaxCols) return DUQ4_ERR_SHAPE;
+    return DUQ4_OK;
+}
+
+template <int SRC>
+static int quantize_rows(int format, int dtype, const RowArgs &a, cudaStream_t st) {
+    if (format == kMX) return dtype == DUQ4_DTYPE_F16 ? launch_rows<SRC, __half, OUT_MX>(a, st) : launch_rows<SRC, __nv_bfloat16, OUT_MX>(a, st);
+    return dtype == DUQ4_DTYPE_F16 ? launch_rows<SRC, __half, OUT_NV>(a, st) : launch_rows<SRC, __nv_bfloat16, OUT_NV>(a, st);
+}
+
+}  // namespace fp4
+}  // namespace duq4
+
+using namespace duq4;
+using namespace duq4::fp4;
+
+extern "C" {
+
+size_t duq4_fp4_scale_bytes(int format, uint32_t rows, uint32_t cols) {
+    if (format != kMX && format != kNV) return 0;
+    return ((size_t)rows + 127) / 128 * scale_tiles(format, cols) * 512;
+}
+
+int duq4_fp4_quantize(int format, int dtype, const void *x, uint32_t rows, uint32_t cols, uint64_t ldx, uint8_t *codes,
+                      uint8_t *block_scales, float *row_scales, void *stream) {
+    DUQ4_TRACE();
+    int rc = check_fp4(format, dtype, cols);
+    if (rc) return rc;
+    if (rows == 0) return DUQ4_OK;
+    if (!x || !codes || !block_scales || (format == kNV && !row_scales)) return DUQ4_ERR_NULL;
+    if (ldx < cols || ldx % 8 != 0) return DUQ4_ERR_SHAPE;
+    if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(block_scales, 16) || !aligned(row_scales, 4)) return DUQ4_ERR_ALIGN;
+    RowArgs a{};
+    a.rows = rows; a.cols = cols; a.ldx = ldx;
+    a.x = (const uint16_t *)x;
+    a.codes = codes; a.block_scales = block_scales; a.row_scales = row_scales;
+    return quantize_rows<SRC_PLAIN>(format, dtype, a, (cudaStream_t)stream);
+}
+
+int duq4_fp4_silu_mul_quantize(int format, int dtype, const void *gate_up, uint32_t rows, uint32_t inter, uint64_t ld, uint32_t up_offset,
+                               uint8_t *codes, uint8_t *block_scales, float *row_scales, void *stream) {
+    DUQ4_TRACE();
+    int rc = check_fp4(format, dtype, inter);
+    if (rc) return rc;
+    if (rows == 0) return DUQ4_OK;
+    if (!gate_up || !codes || !block_scales || (format == kNV && !row_scales)) return DUQ4_ERR_NULL;
+    if (ld % 8 != 0 || up_offset % 8 != 0 || (uint64_t)up_offset + inter > ld) return DUQ4_ERR_SHAPE;
+    if (!aligned(gate_up, 16) || !aligned(codes, 16) || !aligned(block_scales, 16) || !aligned(row_scales, 4)) return DUQ4_ERR_ALIGN;
+    RowArgs a{};
+    a.rows = rows; a.cols = inter; a.ldx = ld; a.up_offset = up_offset;
+    a.x = (const uint16_t *)gate_up;
+    a.codes = codes; a.block_scales = block_scales; a.row_scales = row_scales;
+    return quantize_rows<SRC_SILU>(format, dtype, a, (cudaStream_t)stream);
+}
+
+int duq4_norm_residual_quantize(int format, const duq4_norm_residual *n, uint32_t rows, uint32_t cols, void *out, void *scales,
+                                void *row_scales, void *stream) {
+    DUQ4_TRACE();
+    if (!n) return DUQ4_ERR_NULL;
+    const bool integer = format == DUQ4_MODE_SYM || format == DUQ4_MODE_ASYM, floating = format == kMX || format == kNV;
+    if (format != DUQ4_MODE_NONE && !integer && !floating) return DUQ4_ERR_MODE;
+    int rc = check_fp4(kMX, n->dtype, cols);
+    if (rc) return rc;
+    if (integer && n->dtype != DUQ4_DTYPE_F16) return DUQ4_ERR_MODE;   // the integer formats' scales are fp16
+    if (rows == 0) return DUQ4_OK;
+    if (!n->x || !n->weight || !out || (format != DUQ4_MODE_NONE && !scales) || ((format == kNV || format == DUQ4_MODE_ASYM) && !row_scales))
+        return DUQ4_ERR_NULL;
+    if (n->residual ? !n->residual_out : (n->residual_out || n->post_weight || n->gate)) return DUQ4_ERR_NULL;
+    if (!(n->eps >= 0)) return DUQ4_ERR_SHAPE;
+    const void *must[] = {n->x, n->residual, n->residual_out, n->post_weight, n->gate, n->weight, out};
+    for (const void *p : must)
+        if (!aligned(p, 16)) return DUQ4_ERR_ALIGN;
+    if (!aligned(scales, floating ? 16 : 2) || !aligned(row_scales, format == kNV ? 4 : 2)) return DUQ4_ERR_ALIGN;
+    RowArgs a{};
+    a.rows = rows; a.cols = cols; a.ldx = cols;
+    a.x = (const uint16_t *)n->x;
+    a.residual = (const uint16_t *)n->residual;
+    a.residual_out = (uint16_t *)n->residual_out;
+    a.post_weight = (const uint16_t *)n->post_weight;
+    a.gate = (const uint16_t *)n->gate;
+    a.gate_per_row = n->gate_per_row != 0;
+    a.weight = (const uint16_t *)n->weight;
+    a.residual_scale = n->residual_scale;
+    a.eps = n->eps;
+    a.clip = n->clip_ratio;
+    a.codes = (uint8_t *)out;
+    a.block_scales = (uint8_t *)scales;
+    a.row_scales = row_scales;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (format == DUQ4_MODE_SYM) return launch_rows<SRC_NORM, __half, OUT_SYM>(a, st);
+    if (format == DUQ4_MODE_ASYM) return launch_rows<SRC_NORM, __half, OUT_ASYM>(a, st);
+    if (format == DUQ4_MODE_NONE)
+        return n->dtype == DUQ4_DTYPE_F16 ? launch_rows<SRC_NORM, __half, OUT_ROW>(a, st) : launch_rows<SRC_NORM, __nv_bfloat16, OUT_ROW>(a, st);
+    return quantize_rows<SRC_NORM>(format, n->dtype, a, st);
+}
+
+int duq4_fp4_dequantize(int format, int dtype, const uint8_t *codes, const uint8_t *block_scales, const float *row_scales, uint32_t rows,
+                        uint32_t cols, void *out, void *stream) {
+    DUQ4_TRACE();
+    if (format != kMX && format != kNV) return DUQ4_ERR_MODE;
+    if (dtype != DUQ4_DTYPE_F16 && dtype != DUQ4_DTYPE_BF16 && dtype != DUQ4_DTYPE_F32) return DUQ4_ERR_MODE;
+    if (cols == 0 || cols % 32 != 0) return DUQ4_ERR_SHAPE;
+    if (rows == 0) return DUQ4_OK;
+    if (!codes || !block_scales || !out || (format == kNV && !row_scales)) return DUQ4_ERR_NULL;
+    if (!aligned(codes, 8) || !aligned(out, 16) || !aligned(row_scales, 4)) return DUQ4_ERR_ALIGN;
+    cudaStream_t st = (cudaStream_t)stream;
+    const uint64_t total = (uint64_t)rows * (cols >> 4);
+    const uint32_t grid = (uint32_t)((total + 255) / 256 < 148u * 32u ? (total + 255) / 256 : 148u * 32u);
+    auto go = [&](auto fmt, auto *o) {
+        fp4_dequant_kernel<decltype(fmt)::value><<<grid, 256, 0, st>>>(codes, block_scales, row_scales, rows, cols, o);
+    };
+    auto by_type = [&](auto fmt) {
+        if (dtype == DUQ4_DTYPE_F16) go(fmt, (__half *)out);
+        else if (dtype == DUQ4_DTYPE_BF16) go(fmt, (__nv_bfloat16 *)out);
+        else go(fmt, (float *)out);
+    };
+    if (format == kMX) by_type(std::integral_constant<int, kMX>{});
+    else by_type(std::integral_constant<int, kNV>{});
+    return launch_status();
+}
+
+}  // extern "C"

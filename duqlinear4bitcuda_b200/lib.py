@@ -11,6 +11,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libduq4.so")
 
 MODE_NONE, MODE_SYM, MODE_SYM_DUAL, MODE_ASYM, MODE_ASYM_DUAL = 0, 1, 2, 3, 4
+FP4_MX, FP4_NV = 16, 17
+DTYPE_F16, DTYPE_BF16, DTYPE_F32 = 0, 1, 2
 MODES = {"none": MODE_NONE, "sym": MODE_SYM, "sym_dual": MODE_SYM_DUAL, "asym": MODE_ASYM, "asym_dual": MODE_ASYM_DUAL}
 
 
@@ -40,13 +42,30 @@ class Epilogue(ctypes.Structure):
     ]
 
 
+class NormResidual(ctypes.Structure):
+    """Mirror of `duq4_norm_residual`."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("gate_per_row", ctypes.c_uint32),
+        ("residual_scale", ctypes.c_float),
+        ("clip_ratio", ctypes.c_float),
+        ("eps", ctypes.c_double),
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("post_weight", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("residual_out", ctypes.c_void_p),
+    ]
+
+
 class Duq4Error(RuntimeError):
     def __init__(self, fn, status, text):
         super().__init__(f"{fn} failed with status {status}: {text}")
         self.status = status
 
 
-_vp, _u32, _f32, _sz, _i = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_float, ctypes.c_size_t, ctypes.c_int
+_vp, _u32, _u64, _f32, _sz, _i = ctypes.c_void_p, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_float, ctypes.c_size_t, ctypes.c_int
 
 # name -> argument types (return type is int unless listed in _RESTYPES)
 SIGNATURES = {
@@ -98,12 +117,21 @@ SIGNATURES = {
     "duq4_reduce_dequant_gather": [_vp, _u32, _u32, _u32, _u32, _u32, ctypes.POINTER(Epilogue), _vp, _vp],
     "duq4_linear_w4a4_from_fp16_to_host_rows": [_vp, _vp, _i, _u32, _u32, _u32, _i, _f32, ctypes.POINTER(Epilogue), _u32, _u32,
                                                 ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_uint64), ctypes.c_uint64, _vp, _u32, _vp, _sz, _vp],
+    "duq4_fp4_scale_bytes": [_i, _u32, _u32],
+    "duq4_fp4_quantize": [_i, _i, _vp, _u32, _u32, _u64, _vp, _vp, _vp, _vp],
+    "duq4_fp4_silu_mul_quantize": [_i, _i, _vp, _u32, _u32, _u64, _u32, _vp, _vp, _vp, _vp],
+    "duq4_fp4_dequantize": [_i, _i, _vp, _vp, _vp, _u32, _u32, _vp, _vp],
+    "duq4_norm_residual_quantize": [_i, ctypes.POINTER(NormResidual), _u32, _u32, _vp, _vp, _vp, _vp],
+    "duq4_linear_fp4": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _i, _vp, _u64, _vp],
+    "duq4_linear_fp4_workspace_bytes": [_i, _u32, _u32],
+    "duq4_linear_fp4_from_16bit": [_i, _i, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _u64, _vp, _sz, _vp],
     "duq4_peer_barrier": [ctypes.POINTER(ctypes.c_void_p), _u32, _u32, ctypes.c_uint64, ctypes.c_uint64, _vp],
     "duq4_last_device_status": [_vp, ctypes.POINTER(ctypes.c_int32)],
 }
 _RESTYPES = {"duq4_version": ctypes.c_char_p, "duq4_error_string": ctypes.c_char_p,
              "duq4_linear_from_fp16_workspace_bytes": ctypes.c_size_t, "duq4_gemm_split_scratch_bytes": ctypes.c_size_t,
              "duq4_linear_from_fp16_prelaid_workspace_bytes": ctypes.c_size_t,
+             "duq4_fp4_scale_bytes": ctypes.c_size_t, "duq4_linear_fp4_workspace_bytes": ctypes.c_size_t,
              "duq4_linear_host_staging_bytes": ctypes.c_size_t, "duq4_linear_pipeline_staging_bytes": ctypes.c_size_t}
 
 if not os.path.exists(LIB_PATH):

@@ -93,3 +93,25 @@ def sym_weight_quant(w, scales):
     """round(w / scales) packed as signed int4 (ref: qlinear4bit/nn/linear.py:72-73). Values
     outside [-8, 7] are an error there (pack_i4 asserts) and here."""
     return pack_i4((w / scales).round().to(torch.int8)).cpu()
+
+
+# ---- microscaled 4-bit floating point ----------------------------------------------------
+
+FP4_BLOCK = {"mxfp4": 32, "nvfp4": 16}
+
+
+def fp4_tile_scales(scales: torch.Tensor) -> torch.Tensor:
+    """(new) Block scales as a checkpoint holds them, [rows, blocks] of bytes (uint8, or float8 types by their bits), in the
+    order the fp4 operators take: tiles of 128 rows x 4 blocks, row r of a tile at byte 16 * (r % 32) + 4 * (r // 32).
+    Places beyond the last row and block are zero."""
+    rows, blocks = scales.shape
+    scales = scales.view(torch.uint8)
+    full = scales.new_zeros(-(-rows // 128) * 128, -(-blocks // 4) * 4)
+    full[:rows, :blocks] = scales
+    return full.view(-1, 4, 32, full.shape[1] // 4, 4).permute(0, 3, 2, 1, 4).reshape(-1)
+
+
+def fp4_untile_scales(tiled: torch.Tensor, rows: int, blocks: int) -> torch.Tensor:
+    """(new) The inverse of fp4_tile_scales: uint8 [rows, blocks]."""
+    full = tiled.view(-1, -(-blocks // 4), 32, 4, 4).permute(0, 3, 2, 1, 4)
+    return full.reshape(full.shape[0] * 128, -1)[:rows, :blocks].contiguous()

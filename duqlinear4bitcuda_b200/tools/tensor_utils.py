@@ -27,6 +27,31 @@ class PackedQuantizedTensor:
         return self.quantized_x.dtype
 
 
+class PackedFP4Tensor:
+    """(new) Microscaled 4-bit activations travelling between a quantizer and a linear module: codes uint8 [..., K/2], block
+    scales in the tensor cores' tile order (rows = the product of the leading sizes), row scales float [rows] ("nvfp4") or
+    None ("mxfp4"), and the 16-bit type they were made from."""
+
+    def __init__(self, format: str, codes: torch.Tensor, block_scales: torch.Tensor, row_scales, dtype: torch.dtype):
+        self.format = format
+        self.codes = codes
+        self.block_scales = block_scales
+        self.row_scales = row_scales
+        self.dtype = dtype
+
+    def size(self):
+        return self.codes.size()
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=None):
+        """The values, [..., K]."""
+        v = ops.fp4_dequantize(self.format, _rows(self.codes)[0], self.block_scales, self.row_scales, self.dtype if dtype is None else dtype)
+        return v.view(*self.codes.shape[:-1], -1)
+
+
 def _rows(t):
     """[..., C] -> ([rows, C], leading shape)."""
     return t.view(-1, t.shape[-1]), tuple(t.shape[:-1])

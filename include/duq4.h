@@ -466,6 +466,79 @@ int duq4_quantize_i8_from_stats(int mode, const void *x, uint32_t rows, uint32_t
 int duq4_reduce_dequant_gather(const int32_t *slabs, uint32_t n_slabs, uint32_t rows_per_slab, uint32_t row0, uint32_t rows,
                                uint32_t N, const duq4_epilogue *epi, void *out, void *stream);
 
+/* ---- microscaled 4-bit floating point (no reference counterpart) ------------------------------------------
+ * Elements are e2m1 numbers (0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives), packed like the int4 tensors: element 2j in
+ * the low nibble of byte j. Formats:
+ *   DUQ4_FP4_MX  one e8m0 scale per 32 neighbours of a row: 2^(floor(log2 max|x|) - 2); byte 0 for a block of zeros
+ *   DUQ4_FP4_NV  one e4m3 scale per 16 neighbours and one float per row. Row scale = max|row| / 2688 rounded to bfloat16
+ *                (not below 2^-110); block scale = e4m3(max|block| / (6 * row scale))
+ * and a code is the e2m1 number nearest to x / (block scale [* row scale]), ties to the even code, at most 6. A block that
+ * holds an infinity or a NaN gets a NaN scale and zero codes (all its values read back as NaN) and does not take part in
+ * its row's maximum.
+ * Block scales are kept in the order in which the tensor cores take them: tiles of 128 rows x 4 blocks (512 bytes), row r
+ * of a tile at byte 16 * (r % 32) + 4 * (r / 32), the tiles of a block of rows one behind the other;
+ * duq4_fp4_scale_bytes bytes in all. Scale bytes of columns beyond the row's end must be 0 (the quantizers write them so);
+ * those of rows beyond the last one are not read into any result and are left as they were.
+ * cols / K % 32 == 0; the quantizers take rows of up to 65536 columns. 16-bit tensors are fp16 or bfloat16 (`dtype`). */
+#define DUQ4_FP4_MX 16
+#define DUQ4_FP4_NV 17
+#define DUQ4_DTYPE_F16 0
+#define DUQ4_DTYPE_BF16 1
+#define DUQ4_DTYPE_F32 2
+
+/* Bytes of the block scales of [rows, cols] (0 for an unknown format). */
+size_t duq4_fp4_scale_bytes(int format, uint32_t rows, uint32_t cols);
+/* x [rows, cols], rows ldx elements apart (ldx % 8 == 0) -> codes [rows, cols/2], block scales, row_scales [rows] (DUQ4_FP4_NV
+ * only; else NULL). x, codes and block_scales 16-byte aligned. */
+int duq4_fp4_quantize(int format, int dtype, const void *x, uint32_t rows, uint32_t cols, uint64_t ldx, uint8_t *codes,
+                      uint8_t *block_scales, float *row_scales, void *stream);
+/* The same of h = silu(gate) * up, which is not stored: gate_up [rows, ld], gate in columns [0, inter), up in
+ * [up_offset, up_offset + inter); rounded as F.silu(gate) * up rounds on 16-bit tensors. ld, up_offset % 8 == 0. */
+int duq4_fp4_silu_mul_quantize(int format, int dtype, const void *gate_up, uint32_t rows, uint32_t inter, uint64_t ld, uint32_t up_offset,
+                               uint8_t *codes, uint8_t *block_scales, float *row_scales, void *stream);
+/* Values of a quantized tensor: code * (block scale [* row scale]) in 32 bits, rounded once to `dtype` (also
+ * DUQ4_DTYPE_F32). out [rows, cols], 16-byte aligned. */
+int duq4_fp4_dequantize(int format, int dtype, const uint8_t *codes, const uint8_t *block_scales, const float *row_scales, uint32_t rows,
+                        uint32_t cols, void *out, void *stream);
+
+/* The joint between two blocks of a transformer in one pass over the rows, its result quantized for the next layer:
+ *   y  = x * rms(x) * post_weight      (post_weight NULL: y = x)           rms(t) = 1 / sqrt(mean(t^2) + eps) per row
+ *   r  = residual + residual_scale * (gate * y)   (gate NULL: y)           rounded to 16 bits, stored to residual_out
+ *   h  = r * rms(r) * weight           (residual NULL: r = x)              rounded to 16 bits, then quantized
+ * x, residual, residual_out [rows, cols]; weights [cols]; gate [cols], or [rows, cols] with gate_per_row != 0; all of
+ * `dtype`, dense and 16-byte aligned. residual_out may be residual or x (in place); it is required with residual, and
+ * post_weight and gate without residual are refused (DUQ4_ERR_NULL). The products are rounded one by one in the order
+ * written, in 32 bits; the sums of squares keep their rounding errors, so results equal those of the steps taken one by
+ * one. `format` and the results: DUQ4_MODE_NONE: out = h itself [rows, cols]; DUQ4_MODE_SYM / DUQ4_MODE_ASYM (fp16 only):
+ * out = int4 codes, scales = fp16 [rows], row_scales = fp16 zero-points [rows] (ASYM), as duq4_quantize_{sym,asym}_fused
+ * gives them for h; DUQ4_FP4_*: out = codes, scales = block scales, row_scales = float [rows] (NV). cols % 32 == 0, at
+ * most 65536. */
+typedef struct duq4_norm_residual {
+    int32_t dtype;           /* DUQ4_DTYPE_F16 / BF16 */
+    uint32_t gate_per_row;
+    float residual_scale;
+    float clip_ratio;        /* DUQ4_MODE_SYM only */
+    double eps;              /* >= 0 */
+    const void *x, *residual, *post_weight, *gate, *weight;
+    void *residual_out;
+} duq4_norm_residual;
+int duq4_norm_residual_quantize(int format, const duq4_norm_residual *n, uint32_t rows, uint32_t cols, void *out, void *scales,
+                                void *row_scales, void *stream);
+
+/* out [M, N] = A [M, K] x W [N, K]^T of two tensors of one format, summed in 32 bits, times the token's and the channel's
+ * float factor (A_row_scales [M], W_row_scales [N]; NULL = 1, either format), plus bias [N] (or NULL), rounded once. bias
+ * and out are of `dtype` (fp16 / bfloat16); rows of out are ldo elements apart (0 = N). Codes and block scales 16-byte
+ * aligned. */
+int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales, const float *A_row_scales, const uint8_t *W,
+                    const uint8_t *W_block_scales, const float *W_row_scales, uint32_t M, uint32_t N, uint32_t K, const void *bias, int dtype,
+                    void *out, uint64_t ldo, void *stream);
+/* The same from 16-bit activations x [M, K] (dense): quantized into `workspace` (device memory, 256-byte aligned,
+ * duq4_linear_fp4_workspace_bytes bytes), then multiplied. Calls that share a workspace must not overlap on the GPU. */
+size_t duq4_linear_fp4_workspace_bytes(int format, uint32_t M, uint32_t K);
+int duq4_linear_fp4_from_16bit(int format, int dtype, const void *x, const uint8_t *W, const uint8_t *W_block_scales,
+                               const float *W_row_scales, uint32_t M, uint32_t N, uint32_t K, const void *bias, void *out, uint64_t ldo,
+                               void *workspace, size_t workspace_bytes, void *stream);
+
 /* Device-side barrier across the ranks of an N-sharded layer, on `stream` (no reference counterpart; it
  * brackets the fused all-gather: "everybody has consumed the previous result" / "everybody's block has
  * landed"). flag_ptrs: HOST array of `world` device addresses, entry r = rank r's flag array of `world`

@@ -6,7 +6,7 @@ import sys
 
 import duqlinear4bitcuda_b200 as _impl
 
-for _name in ("_CUDA", "tools", "tools.quantization", "tools.tensor_utils", "nn", "nn.quantizer", "nn.linear", "nn.matmul"):
+for _name in ("_CUDA", "tools", "tools.quantization", "tools.tensor_utils", "nn", "nn.quantizer", "nn.linear", "nn.matmul", "nn.fp4"):
     _mod = importlib.import_module("duqlinear4bitcuda_b200." + _name)
     sys.modules["qlinear4bit." + _name] = _mod
     if "." not in _name:

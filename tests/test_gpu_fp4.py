@@ -1,0 +1,318 @@
+"""Microscaled 4-bit operators against their definitions in 64 bits (tests/_fp4.py)."""
+import numpy as np
+import pytest
+import torch
+
+from tests import _fp4 as F
+
+pytestmark = pytest.mark.gpu
+FORMATS = ["mxfp4", "nvfp4"]
+DTYPES = [torch.float16, torch.bfloat16]
+
+
+def ops():
+    import duqlinear4bitcuda_b200._CUDA as o
+    return o
+
+
+def make(rows, cols, dtype, seed=0, loud=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, cols, generator=g)
+    if loud:
+        x = x * torch.where(torch.rand(cols, generator=g) < 0.02, 30.0, 1.0) * torch.exp(torch.randn(rows, 1, generator=g))
+    return x.to(dtype)
+
+
+def check_quantized(fmt, got, x64):
+    """Codes, block scales (in place and zero in the padding columns) and row scales are those of the definition, exactly."""
+    codes, tiled, rows = got
+    c, b, r = F.quantize(fmt, x64)
+    n, blocks = b.shape
+    g = codes.cpu().numpy()
+    t = tiled.cpu().numpy()
+    assert np.array_equal(F.untile(t, n, blocks), b)
+    padded = -(-blocks // 4) * 4
+    assert not F.untile(t, n, padded)[:, blocks:].any()
+    assert np.array_equal(F.unpack(g), c)
+    if fmt == "nvfp4":
+        assert np.array_equal(rows.cpu().numpy().astype(np.float64), r)
+    else:
+        assert rows is None
+
+
+SIZES = [(1, 32), (1, 4096), (3, 64), (5, 96), (128, 160), (129, 224), (33, 2080), (7, 8192), (2, 11008), (3, 16416), (2, 33024), (1, 65536)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", SIZES)
+def test_quantize(fmt, dtype, rows, cols):
+    x = make(rows, cols, dtype, rows + cols)
+    check_quantized(fmt, ops().fp4_quantize(fmt, x.cuda()), x.double().numpy())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_quantize_every_half(fmt):
+    """Every finite fp16 number as an element, beside tops of every exponent: all roundings and ties."""
+    bits = torch.arange(0, 0x7C00, dtype=torch.int32)
+    x = bits.to(torch.int16).view(torch.float16)
+    x = torch.cat([x, -x])[:63488].reshape(-1, 64).clone()
+    x = torch.cat([x, x[torch.randperm(x.shape[0], generator=torch.Generator().manual_seed(1))].reshape(64, -1).t().contiguous().view(-1, 64)])
+    check_quantized(fmt, ops().fp4_quantize(fmt, x.cuda()), x.double().numpy())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_special_rows(fmt, dtype):
+    """Zero rows and blocks, the smallest and largest numbers, infinities and NaNs: a bad block reads back as NaN, the others
+    of its row as if it were zero."""
+    x = make(12, 256, dtype, 3)
+    x[0] = 0
+    x[1] = 0
+    x[1, 255] = torch.finfo(dtype).smallest_normal
+    x[2] = torch.finfo(dtype).max
+    x[3, :16] = 0
+    x[4, 5] = float("inf")
+    x[5, 40] = float("nan")
+    x[6, 70] = -float("inf")
+    x[7] = float("nan")
+    x[8] = -torch.finfo(dtype).tiny * torch.finfo(dtype).eps   # the smallest subnormal
+    x[9] = torch.finfo(dtype).smallest_normal
+    x[10, ::2] = -0.0
+    got = ops().fp4_quantize(fmt, x.cuda())
+    check_quantized(fmt, got, x.double().numpy())
+    back = ops().fp4_dequantize(fmt, *got, torch.float32).cpu()
+    want = torch.from_numpy(F.values(fmt, *F.quantize(fmt, x.double().numpy())).astype(np.float32))
+    assert torch.equal(back.isnan(), want.isnan())
+    assert torch.allclose(back.nan_to_num(), want.nan_to_num(), rtol=2 ** -22, atol=0)
+    assert back[4, :16].isnan().all() and not back[4, 32:].isnan().any()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 32), (130, 96), (5, 4128)])
+def test_dequantize(fmt, dtype, rows, cols):
+    packed, tiled, row, v = F.random_operand(fmt, rows, cols, rows)
+    if fmt == "mxfp4":
+        row, v = None, v / row[:, None]
+    got = ops().fp4_dequantize(fmt, F.cuda(packed), F.cuda(tiled), F.cuda(row), dtype).double().cpu().numpy()
+    # half a step of the result's type on top of the one rounding of block scale * row scale and of its product
+    tol = torch.finfo(dtype).eps / 2 + 2 * 2.0 ** -24
+    assert np.all(np.abs(got - v) <= tol * np.abs(v) * (1 + 2.0 ** -10) + (2.0 ** -25 if dtype == torch.float16 else 0))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,inter", [(1, 32), (16, 11008), (131, 96), (3, 28672)])
+def test_silu_mul_quantize_equals_the_composition(fmt, dtype, rows, inter):
+    gu = (make(rows, 2 * inter, dtype, 5, loud=False) * 2).cuda()
+    h = torch.nn.functional.silu(gu[:, :inter]) * gu[:, inter:]
+    a, b = ops().fp4_silu_mul_quantize(fmt, gu), ops().fp4_quantize(fmt, h)
+    assert torch.equal(a[0], b[0])
+    blocks = inter // F.BLOCK[fmt]
+    assert np.array_equal(F.untile(a[1].cpu().numpy(), rows, blocks), F.untile(b[1].cpu().numpy(), rows, blocks))
+    assert a[2] is None if fmt == "mxfp4" else torch.equal(a[2], b[2])
+
+
+def _norm(t, w, eps):
+    """fp32 steps of x * rms(x) * w with the mean in 64 bits."""
+    d = t.double()
+    rstd = (1.0 / torch.sqrt((d * d).mean(-1, keepdim=True) + eps)).float()
+    return t.float() * rstd * w.float()
+
+
+def _joint(x, weight, eps, residual, post, gate, scale):
+    y = x.float()
+    if residual is None:
+        r = x
+    else:
+        if post is not None:
+            y = _norm(x, post, eps)
+        if gate is not None:
+            y = y * gate.float()
+        r = (residual.float() + y * scale).to(x.dtype)
+    return r, _norm(r, weight, eps).to(x.dtype)
+
+
+@pytest.mark.parametrize("fmt", ["none", "sym", "asym", "mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(1, 32), (1, 4096), (5, 96), (130, 2080), (3, 8192), (2, 16448), (1, 65536)])
+@pytest.mark.parametrize("form", ["pre", "residual", "post", "gate", "gate_row", "all"])
+def test_norm_residual_quantize_equals_its_steps(fmt, dtype, rows, cols, form):
+    if fmt in ("sym", "asym") and (dtype != torch.float16 or cols > 32768):
+        pytest.skip("integer formats: fp16, and the quantizer compared with takes 32768 columns in the same arithmetic")
+    x, residual = make(rows, cols, dtype, 1).cuda(), make(rows, cols, dtype, 2).cuda()
+    weight, post = (1 + 0.1 * make(1, cols, torch.float32, 3, False)[0]).to(dtype).cuda(), make(1, cols, dtype, 4, False)[0].cuda()
+    gate = make(rows, cols, dtype, 5, False).cuda() if form == "gate_row" else make(1, cols, dtype, 6, False)[0].cuda()
+    res = None if form == "pre" else residual
+    post = post if form in ("post", "all") else None
+    gate = gate if form in ("gate", "gate_row", "all") else None
+    scale = 1.0 if form in ("pre", "residual") else 0.37
+    r, h = _joint(x, weight, 1e-5, res, post, gate, scale)
+    got_r, *got = ops().norm_residual_quantize(fmt, x, weight, 1e-5, res, post, gate, scale)
+    assert got_r is None if res is None else torch.equal(got_r, r)
+    if fmt == "none":
+        assert torch.equal(got[0], h)
+        return
+    want = {"sym": lambda: ops().quantize_sym_fused(h), "asym": lambda: ops().quantize_asym_fused(h)}.get(fmt, lambda: ops().fp4_quantize(fmt, h))()
+    assert torch.equal(got[0], want[0])
+    if fmt in ("sym", "asym"):
+        assert all(torch.equal(a, b) for a, b in zip(got[1:], want[1:]))
+        return
+    blocks = cols // F.BLOCK[fmt]
+    assert np.array_equal(F.untile(got[1].cpu().numpy(), rows, blocks), F.untile(want[1].cpu().numpy(), rows, blocks))
+    assert got[2] is None if fmt == "mxfp4" else torch.equal(got[2], want[2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norm_of_extreme_rows(dtype):
+    """Rows of zeros, of the smallest and the largest numbers, with an infinity, with a NaN."""
+    big = torch.finfo(dtype).max
+    x = torch.zeros(6, 96, dtype=dtype)
+    x[1] = torch.finfo(dtype).smallest_normal
+    x[2] = big
+    x[3] = make(1, 96, dtype)[0]
+    x[3, 7] = float("inf")
+    x[4] = make(1, 96, dtype)[0]
+    x[4, 90] = float("nan")
+    x[5] = torch.linspace(-1, 1, 96).to(dtype) * (big / 4)
+    w = torch.ones(96, dtype=dtype)
+    for eps in (0.0, 1e-6):
+        want = _joint(x, w, eps, None, None, None, 1.0)[1]
+        got = ops().norm_residual_quantize("none", x.cuda(), w.cuda(), eps)[1].cpu()
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+def check_product(got, a, w, bias, dtype):
+    """|y - exact| within half a step of the type and the rounding of a 32-bit sum of K products: each product of two codes and
+    the sum's terms are exact, the terms' running sum is rounded (or cut off) at most once per addition, so the error is
+    at most K steps of 2^-23 of the sum of magnitudes; a few more roundings for the factors."""
+    exact = a @ w.T + (0 if bias is None else bias)
+    mags = np.abs(a) @ np.abs(w).T + (0 if bias is None else np.abs(bias))
+    k = a.shape[1]
+    tol = torch.finfo(dtype).eps / 2 * np.abs(exact) * (1 + 2.0 ** -7) + (k + 8) * 2.0 ** -23 * mags
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25
+    off = np.abs(got.double().cpu().numpy() - exact)
+    assert np.all(off <= tol), (np.nanmax(off / tol), np.argwhere(~(off <= tol))[:5])
+
+
+PRODUCTS = [(1, 8, 32), (1, 129, 96), (2, 256, 256), (3, 100, 288), (8, 1024, 512), (16, 130, 4096), (17, 33, 1056), (32, 512, 11008), (33, 384, 640),
+            (77, 300, 1120), (128, 256, 1024), (129, 257, 544), (200, 1000, 320), (256, 512, 2048), (300, 384, 64), (513, 700, 96), (640, 640, 1312)]
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+@pytest.mark.parametrize("form", ["plain", "rows", "bias"])
+def test_linear_fp4(fmt, m, n, k, form):
+    dtype = torch.bfloat16 if (m + n) % 2 else torch.float16
+    ap, at, ar, av = F.random_operand(fmt, m, k, m + n + k, form != "plain")
+    wp, wt, wr, wv = F.random_operand(fmt, n, k, m * n + k, form != "plain")
+    scale = 1.0 if dtype == torch.bfloat16 else 2.0 ** -12   # results inside fp16
+    if form == "plain" and dtype == torch.float16:
+        wr, wv = np.full(n, scale / (1 if fmt == "mxfp4" else 64), np.float32), wv * (scale / (1 if fmt == "mxfp4" else 64))
+    elif dtype == torch.float16 and fmt == "mxfp4":
+        wr, wv = wr * np.float32(scale), wv * scale
+    bias = make(1, n, dtype, 9)[0] if form == "bias" else None
+    got = ops().linear_fp4(fmt, F.cuda(ap), F.cuda(at), F.cuda(ar), F.cuda(wp), F.cuda(wt), F.cuda(wr), None if bias is None else bias.cuda(), dtype)
+    assert got.shape == (m, n) and got.dtype == dtype
+    check_product(got, av, wv, None if bias is None else bias.double().numpy(), dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (5, 70, 96), (16, 640, 1024), (40, 512, 512), (150, 384, 1376), (520, 1030, 512)])
+def test_linear_from_16bit_equals_quantizer_and_product(fmt, dtype, m, n, k):
+    x = make(m, k, dtype, 7).cuda()
+    wp, wt, wr, _ = F.random_operand(fmt, n, k, 11)
+    w = (F.cuda(wp), F.cuda(wt), F.cuda(wr))
+    bias = make(1, n, dtype, 9)[0].cuda()
+    want = ops().linear_fp4(fmt, *ops().fp4_quantize(fmt, x), *w, bias, dtype)
+    assert torch.equal(ops().linear_fp4_from_16bit(fmt, x, *w, bias), want)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [3, 150])
+def test_a_bad_token_spoils_its_own_row_only(fmt, m):
+    """Infinities and NaNs in one token's activations: its row of the result is NaN, every other row as without them."""
+    x = make(m, 256, torch.bfloat16, 7).cuda()
+    wp, wt, wr, _ = F.random_operand(fmt, 200, 256, 11)
+    w = (F.cuda(wp), F.cuda(wt), F.cuda(wr))
+    clean = ops().linear_fp4_from_16bit(fmt, x, *w)
+    x[1, 100], x[2, 3] = float("nan"), float("-inf")
+    got = ops().linear_fp4_from_16bit(fmt, x, *w)
+    assert got[1:3].isnan().all()
+    keep = [i for i in range(m) if i not in (1, 2)]
+    assert torch.equal(got[keep], clean[keep])
+
+
+def test_empty_batches():
+    o = ops()
+    for fmt in FORMATS:
+        x = torch.empty(0, 64, dtype=torch.float16, device="cuda")
+        q = o.fp4_quantize(fmt, x)
+        assert q[0].shape == (0, 32) and o.fp4_dequantize(fmt, *q, torch.float16).shape == (0, 64)
+        wp, wt, wr, _ = F.random_operand(fmt, 40, 64, 1)
+        assert o.linear_fp4_from_16bit(fmt, x, F.cuda(wp), F.cuda(wt), F.cuda(wr)).shape == (0, 40)
+        assert o.norm_residual_quantize(fmt, x, torch.ones(64, dtype=torch.float16, device="cuda"))[1].shape == (0, 32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("tokens", [1, 19, 300])
+def test_mlp_block_of_modules(fmt, tokens):
+    """The operators as they are used: norm -> gate/up layer -> SiLU product -> down layer -> norm after the block, residual
+    sum, next norm, quantized. Every stage equals the same stage from its 16-bit or read-back inputs; graph replay too."""
+    import duqlinear4bitcuda_b200.nn as nn
+    g = torch.Generator().manual_seed(tokens)
+    dim, inter, dtype = 256, 416, torch.bfloat16
+    lin = lambda i, o: torch.nn.Linear(i, o, bias=True).to(dtype).cuda()
+    gate_up, down = lin(dim, 2 * inter), lin(inter, dim)
+    first, last = nn.NormResidualQuantizer(dim, fmt, dtype=dtype).cuda(), nn.NormResidualQuantizer(dim, fmt, post_norm=True, residual_scale=0.5, dtype=dtype).cuda()
+    q_gate_up, q_down = nn.LinearFP4.from_linear(gate_up, fmt, dtype), nn.LinearFP4.from_linear(down, fmt, dtype)
+    glue = nn.SiluMulQuantizerFP4(fmt)
+    x = torch.randn(1, tokens, dim, generator=g).to(dtype).cuda()
+    gate = torch.randn(1, tokens, dim, generator=g).to(dtype).cuda()
+
+    def block(x):
+        h = first(x)
+        y = q_gate_up(h)
+        a = glue(y)
+        z = q_down(a)
+        return h, y, a, z, *last(z, x, gate)
+    h, y, a, z, nxt, stream = block(x)
+    assert nxt.size() == (1, tokens, dim // 2) and stream.shape == x.shape
+    assert torch.equal(q_gate_up(first(x)), y)
+    check_product(y[0], h.dequantize(torch.float32)[0].double().cpu().numpy(),
+                  _weights64(q_gate_up), q_gate_up.bias.double().cpu().numpy(), dtype)
+    check_product(z[0], a.dequantize(torch.float32)[0].double().cpu().numpy(), _weights64(q_down), q_down.bias.double().cpu().numpy(), dtype)
+    r, hn = _joint(z[0], last.weight, last.eps, x[0], last.post_weight, gate[0], 0.5)
+    assert torch.equal(stream[0], r)
+    assert torch.equal(nxt.codes[0], ops().fp4_quantize(fmt, hn)[0])
+    # two captures replayed in turn give the eager results
+    xs, outs, graphs = [x.clone(), x.flip(-1).contiguous()], [], []
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        block(x)
+    torch.cuda.current_stream().wait_stream(side)
+    for t in xs:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            res = block(t)
+            outs.append((res[3], res[5], res[4].codes))
+        graphs.append(gr)
+    for _ in range(2):
+        for gr in graphs:
+            gr.replay()
+    torch.cuda.synchronize()
+    for t, got in zip(xs, outs):
+        want = block(t)
+        assert torch.equal(got[0], want[3]) and torch.equal(got[1], want[5]) and torch.equal(got[2], want[4].codes)
+
+
+def _weights64(layer):
+    rows, cols = layer.out_features, layer.in_features
+    byte = F.untile(layer.weight_scales.cpu().numpy(), rows, cols // F.BLOCK[layer.format])
+    row = None if layer.weight_row_scales is None else layer.weight_row_scales.cpu().numpy()
+    return F.values(layer.format, F.unpack(layer.weight.cpu().numpy()), byte, row)
