@@ -27,6 +27,7 @@ int tc_status_read(cudaStream_t st, int32_t *out);
 int gemv_status_read(int32_t *out);
 int peer_status_read(int32_t *out);
 int tc2_status_read(int32_t *out);
+int fp4_status_read(int32_t *out);
 extern std::atomic<int> g_static_weights;
 int quantize_fused_dispatch(int mode, const void *x, uint32_t rows, uint32_t cols, float clip, uint8_t *q, void *s1,
                             void *z1, void *s2, void *z2, cudaStream_t st, bool out8);
@@ -407,8 +408,11 @@ int duq4_last_device_status(void *stream, int32_t *status_out) {
     int32_t d = 0;
     rc = peer_status_read(&d);
     if (rc) return rc;
-    // 1..9: tensor-core GEMM wait, 101..: small-M kernel wait, 201..: CTA-pair GEMM wait, 301: peer barrier wait
-    *status_out = a ? a : (b ? 100 + b : (c ? 200 + c : (d ? 300 + d : 0)));
+    int32_t f = 0;
+    rc = fp4_status_read(&f);
+    if (rc) return rc;
+    // 1..9: tensor-core GEMM wait, 101..: small-M kernel wait, 201..: CTA-pair GEMM wait, 301: peer barrier wait, 401..: fp4 product wait
+    *status_out = a ? a : (b ? 100 + b : (c ? 200 + c : (d ? 300 + d : (f ? 400 + f : 0))));
     return DUQ4_OK;
 }
 

@@ -1,10 +1,29 @@
 // Product of two microscaled 4-bit matrices, Y[M,N] = A[M,K] * W[N,K]^T, with the per-token and per-channel factors and
 // the bias in the epilogue. No counterpart in the reference.
+//
+// The tensor cores take the format as it is: tcgen05.mma with block scaling multiplies packed e2m1 operands from shared
+// memory (64 columns of K per instruction) and takes each block's scale from TMEM. A stage of either kernel is 256 columns
+// of K: 128-byte rows of codes (128-byte swizzle) and the scale tiles that go with them, all brought by TMA; tcgen05.cp
+// then spreads each 512-byte scale tile (128 rows x 4 blocks) over four TMEM columns. Copies and MMAs are issued by one
+// thread and execute in its order, so one set of TMEM columns for the scales serves all stages.
+//
+//   fp4_pair_kernel   many tokens: CTA pairs, 256 tokens x 256 (128) channels per tile, one persistent pair per two SMs
+//   fp4_swap_kernel   few tokens: the weights are the 128-row operand and the tokens (16 .. 128) the MMA's N, so that a
+//                     decode step streams weights and wastes no MMA on absent tokens; K is split over a cluster
+#include <cuda.h>
+
 #include "fp4_common.cuh"
+#include "gemm_tc_shared.cuh"
 #include "trace_range.h"
 
 namespace duq4 {
+
+__device__ int g_fp4_status = 0;
+
 namespace fp4 {
+
+using namespace ptx;
+using namespace tc;
 
 struct GemmArgs {
     uint32_t M, N, K;
@@ -15,69 +34,600 @@ struct GemmArgs {
     uint64_t ldo;
 };
 
-// y = acc * token factor * channel factor + bias, rounded once
-template <class T>
-__device__ __forceinline__ uint16_t finish(float acc, float ra, float rw, float b) {
-    return (uint16_t)(Two<T>::down(__fmaf_rn(__fmul_rn(acc, ra), rw, b), 0.f) & 0xFFFFu);
+constexpr int kBK = 256;            // K per stage: 128 bytes of codes per row
+constexpr int kTileBytes = 512;     // scale tile: 128 rows x 4 blocks
+
+__device__ __forceinline__ void fp4_fail(volatile int *abort_flag, int code) {
+    *abort_flag = 1;
+    atomicCAS(&g_fp4_status, 0, code);
+}
+// Bounded wait on a barrier of this CTA (arrivals may come from the partner).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int code) {
+    return mbar_wait(bar, parity, abort_flag, &g_fp4_status, code);
 }
 
-// 64 x 64 outputs per CTA, 32 columns of K at a time as floats in shared memory.
-template <int FMT, class T>
-__global__ void __launch_bounds__(256) fp4_gemm_simt_kernel(const GemmArgs a) {
-    __shared__ float sa[32][65], sw[32][65];
-    const uint32_t m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, tiles = scale_tiles(FMT, a.K);
-    const uint32_t tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    for (uint32_t k0 = 0; k0 < a.K; k0 += 32) {
-        // 128 rows (64 of A, 64 of W), two threads each, 16 columns per thread
-        const uint32_t r = threadIdx.x >> 1, half = threadIdx.x & 1, lr = r & 63;
-        const bool is_w = r >= 64;
-        const uint32_t row = (is_w ? n0 : m0) + lr, k = k0 + half * 16;
-        float (*dst)[65] = is_w ? sw : sa;
-        uint2 w = make_uint2(0, 0);
-        float s = 0.f;
-        if (row < (is_w ? a.N : a.M)) {
-            w = *reinterpret_cast<const uint2 *>((is_w ? a.w : a.a) + (size_t)row * (a.K >> 1) + (k >> 1));
-            const uint32_t blk = k / block_of(FMT);
-            s = block_scale_to_float<FMT>((is_w ? a.w_scales : a.a_scales)[scale_offset(tiles, row, blk >> 2) + (blk & 3)]);
-        }
+// Instruction descriptor of the block-scaled kinds: e2m1 x e2m1 -> f32, both operands K-major. `sf`: which bytes of the
+// 32-bit scale words the instruction takes (0 or 2; two scales per instruction of the 32-blocks, four of the 16-blocks).
+template <int FMT>
+__device__ __forceinline__ uint32_t block_idesc(int m, uint32_t n, uint32_t sf) {
+    return (sf << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((FMT == kMX ? 1u : 0u) << 23) | ((uint32_t)(m >> 4) << 24) | (sf << 29);
+}
+// Scale tile in shared memory for tcgen05.cp: 8 rows of 16 bytes are contiguous, groups of 8 rows 128 bytes apart.
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 | (uint64_t)(128u >> 4) << 32 | (uint64_t)1 << 46;
+}
+template <int CG>
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
+    if (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+#define DUQ4_FP4_MMA(GROUP, KIND)                                                                                          \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                                           \
+                 "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%4], [%5], p;\n\t}"                     \
+                 ::"r"(d), "l"(da), "l"(db), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory")
+template <int FMT, int CG>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    if (FMT == kMX && CG == 2) DUQ4_FP4_MMA("2", "mxf4.block_scale.scale_vec::2X");
+    if (FMT == kMX && CG == 1) DUQ4_FP4_MMA("1", "mxf4.block_scale.scale_vec::2X");
+    if (FMT == kNV && CG == 2) DUQ4_FP4_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    if (FMT == kNV && CG == 1) DUQ4_FP4_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X");
+}
+#undef DUQ4_FP4_MMA
+
+// One stage: its scale tiles to TMEM, its four MMAs. Scale tiles lie [block of 128 rows][tile] in shared memory and
+// [tile][block of rows] in TMEM (four columns each), so that the rows of one MMA are contiguous. a_blocks, b_blocks:
+// 128-row blocks of either operand in this CTA's shared memory.
+template <int FMT, int CG>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint32_t sa, uint32_t sb, uint32_t ssa, uint32_t ssb, uint32_t ta, uint32_t tb,
+                                            uint32_t b_blocks, int m, uint32_t n, bool first) {
+    constexpr int kTiles = kBK / (4 * (int)block_of(FMT));   // 2 or 4 scale tiles per stage and block of rows
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float2 f = __half22float2(e2m1x2_to_half2((j < 4 ? w.x : w.y) >> (8 * (j & 3)) & 0xFFu));
-            dst[half * 16 + 2 * j][lr] = f.x * s;
-            dst[half * 16 + 2 * j + 1][lr] = f.y * s;
-        }
-        __syncthreads();
-#pragma unroll 8
-        for (int kk = 0; kk < 32; ++kk) {
-            float x[4], y[4];
+    for (int j = 0; j < kTiles; ++j) copy_scales<CG>(ta + j * 4, scale_desc(ssa + j * kTileBytes));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { x[i] = sa[kk][ty * 4 + i]; y[i] = sw[kk][tx * 4 + i]; }
+    for (int j = 0; j < kTiles; ++j)
+        for (uint32_t b = 0; b < b_blocks; ++b)
+            copy_scales<CG>(tb + (j * b_blocks + b) * 4, scale_desc(ssb + (b * kTiles + j) * kTileBytes));
+    const uint64_t da = make_desc(sa), db = make_desc(sb);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
-        }
-        __syncthreads();
+    for (int kk = 0; kk < 4; ++kk) {
+        const int j = FMT == kMX ? kk >> 1 : kk;
+        const uint32_t sf = FMT == kMX ? (kk & 1) * 2 : 0;
+        mma<FMT, CG>(d, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), block_idesc<FMT>(m, n, sf), ta + j * 4, tb + j * b_blocks * 4,
+                     !first || kk > 0);
     }
+}
+
+// y = acc * token factor * channel factor + bias
+__device__ __forceinline__ float finish(float acc, float ra, float rw, float b) { return __fmaf_rn(__fmul_rn(acc, ra), rw, b); }
+
+__device__ __forceinline__ uint32_t ctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t local_addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(local_addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t cluster_bar) {
+    if (CG == 2) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_bar) : "memory");
+    else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cluster_bar) : "memory");
+}
+// Copies whose bytes are credited to a barrier of either CTA of the pair (CG == 2) or of this CTA.
+template <int CG>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y) {
+    if (CG == 2)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                     "l"(map), "r"(bar), "r"(x), "r"(y) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(map),
+                     "r"(bar), "r"(x), "r"(y) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
+    if (CG == 2)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+                     "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z) : "memory");
+    else
+        tma_load_3d(dst, map, bar, x, y, z);
+}
+__device__ __forceinline__ void leave_copies_behind() {   // a producer that gives up lets its copies land first
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
+}
+
+// ---- many tokens: CTA pairs -------------------------------------------------------------------------------------
+struct PairArgs {
+    GemmArgs g;
+    uint32_t tiles_m, tiles_n, bn;   // tiles of 256 tokens x bn channels (128 or 256)
+};
+
+template <int FMT>
+struct Pair {
+    static constexpr int kTiles = kBK / (4 * (int)block_of(FMT));
+    static constexpr int kStages = FMT == kMX ? 6 : 5;
+    static constexpr int kOperand = 128 * 128;                 // one CTA's 128 rows of codes
+    static constexpr int kScaleA = kTiles * kTileBytes, kScaleStage = 3 * kScaleA;   // own tokens, then all channels of the tile
+    static constexpr int kSmem = 1024 + kStages * (2 * kOperand + kScaleStage);
+    static constexpr int kThreads = 32 * 10;
+    // TMEM: two accumulators of 256 columns and the scales do not fit in 512 columns side by side, so the second
+    // accumulator starts inside the first: its first 64 columns are the first one's last 64. The epilogue takes those
+    // columns first and lets the next tile start when it has them in registers.
+    static constexpr uint32_t kSecond = 192, kSfa = 448, kSfb = 448 + 4 * kTiles;
+    static_assert(kSfb + 8 * kTiles <= 512 && kSmem <= 232448 - 512, "does not fit");
+};
+
+// 32 neighbouring channels of one token from the accumulator to memory.
+template <class T>
+__device__ __forceinline__ void store32(const GemmArgs &a, const uint32_t (&v)[32], uint32_t m, uint32_t n, float ra, bool vec) {
+    uint16_t *row = reinterpret_cast<uint16_t *>(a.out) + (size_t)m * a.ldo + n;
+    const uint16_t *bias = reinterpret_cast<const uint16_t *>(a.bias);
+    if (vec && n + 32 <= a.N) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int q = 0; q < 4; ++q) {
+            float y[8];
+            if (a.w_rows) {
+                const float4 s0 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n + q * 8)), s1 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n + q * 8) + 1);
+                const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-            if (m >= a.M || n >= a.N) continue;
-            const float b = a.bias ? Two<T>::up1(reinterpret_cast<const uint16_t *>(a.bias)[n]) : 0.f;
-            reinterpret_cast<uint16_t *>(a.out)[m * a.ldo + n] =
-                finish<T>(acc[i][j], a.a_rows ? a.a_rows[m] : 1.f, a.w_rows ? a.w_rows[n] : 1.f, b);
+                for (int j = 0; j < 8; ++j) y[j] = s[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) y[j] = 1.f;
+            }
+            uint4 b = make_uint4(0, 0, 0, 0);
+            if (bias) b = __ldg(reinterpret_cast<const uint4 *>(bias + n + q * 8));
+            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 bf = Two<T>::up(bw[j]);
+                o[j] = Two<T>::down(finish(__uint_as_float(v[q * 8 + 2 * j]), ra, y[2 * j], bf.x),
+                                    finish(__uint_as_float(v[q * 8 + 2 * j + 1]), ra, y[2 * j + 1], bf.y));
+            }
+            reinterpret_cast<uint4 *>(row)[q] = make_uint4(o[0], o[1], o[2], o[3]);
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+            if (n + j < a.N)
+                row[j] = (uint16_t)(Two<T>::down(finish(__uint_as_float(v[j]), ra, a.w_rows ? a.w_rows[n + j] : 1.f,
+                                                        bias ? Two<T>::up1(bias[n + j]) : 0.f), 0.f) & 0xFFFFu);
+    }
 }
 
 template <int FMT, class T>
-static int gemm(const GemmArgs &a, cudaStream_t st) {
-    const dim3 grid(cdiv(a.N, 64), cdiv(a.M, 64));
-    if (grid.y > 65535) return DUQ4_ERR_SHAPE;
-    fp4_gemm_simt_kernel<FMT, T><<<grid, 256, 0, st>>>(a);
+__global__ void __launch_bounds__(Pair<FMT>::kThreads, 1)
+fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sa,
+                const __grid_constant__ CUtensorMap map_sw, const PairArgs p) {
+    using C = Pair<FMT>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    __shared__ __align__(8) uint64_t bars[2 * C::kStages + 6];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, scales0 = base + C::kStages * 2 * C::kOperand, bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };                        // the leader's: both CTAs' copies
+    auto empty = [&](int s) { return bar0 + 8u * (C::kStages + s); };        // each CTA's: the MMAs that read the stage
+    auto acc_full = [&](int b) { return bar0 + 8u * (2 * C::kStages + b); }; // each CTA's
+    auto acc_empty = [&](int b) { return bar0 + 8u * (2 * C::kStages + 2 + b); };   // the leader's: epilogue warps of both
+    const uint32_t shared_free = bar0 + 8u * (2 * C::kStages + 4);           // the leader's: the shared columns are read
+    const uint32_t drained = bar0 + 8u * (2 * C::kStages + 5);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = ctarank(), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const uint32_t tiles = p.tiles_m * p.tiles_n, ksteps = (p.g.K + kBK - 1) / kBK, bn = p.bn;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), 16);
+        }
+        mbar_init(shared_free, 16);
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&tmem_slot)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+    volatile int *abortp = &abort_flag;
+
+    // Tile order: token blocks fastest inside bands of 16, so that the pairs at work share a few weight tiles and a band of
+    // activations that stays in L2.
+    auto coords = [&](uint32_t t, uint32_t &tm, uint32_t &tn) {
+        const uint32_t per_band = 16 * p.tiles_n, band = t / per_band, r = t % per_band, here = min(16u, p.tiles_m - band * 16);
+        tn = r / here;
+        tm = band * 16 + r % here;
+    };
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            const uint32_t bytes = 2 * (C::kOperand + bn / 2 * 128 + C::kScaleA * (1 + bn / 128));
+            for (uint32_t t = pair; ok && t < tiles; t += npairs) {
+                uint32_t tm, tn;
+                coords(t, tm, tn);
+                for (uint32_t ks = 0; ks < ksteps; ++ks, ++it) {
+                    const uint32_t s = it % C::kStages, ph = (it / C::kStages) & 1;
+                    if (!(ok = wait(empty(s), ph ^ 1, abortp, 1))) break;
+                    if (rank == 0) mbar_expect_tx(full(s), bytes);
+                    const uint32_t bar = in_cta(full(s), 0), dst = base + s * 2 * C::kOperand, sc = scales0 + s * C::kScaleStage;
+                    load_2d<2>(dst, &map_a, bar, ks * 128, tm * 256 + rank * 128);
+                    load_2d<2>(dst + C::kOperand, &map_w, bar, ks * 128, tn * bn + rank * (bn / 2));
+                    load_3d<2>(sc, &map_sa, bar, 0, ks * C::kTiles, tm * 2 + rank);
+                    load_3d<2>(sc + C::kScaleA, &map_sw, bar, 0, ks * C::kTiles, tn * (bn / 128));
+                }
+            }
+            if (!ok) leave_copies_behind();
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t it = 0, lt = 0;
+            bool ok = true, issued = false;
+            for (uint32_t t = pair; ok && t < tiles; t += npairs, ++lt) {
+                const uint32_t buf = lt & 1;
+                if (!(ok = wait(acc_empty(buf), ((lt >> 1) & 1) ^ 1, abortp, 2))) break;
+                if (lt > 0 && !(ok = wait(shared_free, (lt - 1) & 1, abortp, 3))) break;
+                tc_fence_after();
+                for (uint32_t ks = 0; ks < ksteps; ++ks, ++it) {
+                    const uint32_t s = it % C::kStages, ph = (it / C::kStages) & 1;
+                    if (!(ok = wait(full(s), ph, abortp, 4))) break;
+                    tc_fence_after();
+                    const uint32_t sa = base + s * 2 * C::kOperand, sc = scales0 + s * C::kScaleStage;
+                    issue_stage<FMT, 2>(tmem + buf * C::kSecond, sa, sa + C::kOperand, sc, sc + C::kScaleA, tmem + C::kSfa, tmem + C::kSfb, bn / 128,
+                                        256, bn, ks == 0);
+                    issued = true;
+                    commit<2>(empty(s));
+                    commit<2>(in_cta(empty(s), 1));
+                }
+                if (ok) {
+                    commit<2>(acc_full(buf));
+                    commit<2>(in_cta(acc_full(buf), 1));
+                }
+            }
+            if (!ok && issued) {
+                commit<2>(drained);
+                const uint64_t t0 = globaltimer();
+                while (!mbar_try(drained, 0) && globaltimer() - t0 < kPtxWaitLimitNs) __nanosleep(1000);
+            }
+        }
+    } else {
+        // Epilogue, eight warps: two per TMEM lane quadrant, which take the tile's 32-column chunks in turn, the shared
+        // ones (6, 7 of the first accumulator, 0, 1 of the second) first.
+        const int quad = warp & 3, half = (warp - 2) >> 2;
+        const bool vec = (p.g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0 &&
+                         (reinterpret_cast<uintptr_t>(p.g.w_rows) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.g.bias) & 15) == 0;
+        uint32_t lt = 0;
+        for (uint32_t t = pair; t < tiles; t += npairs, ++lt) {
+            uint32_t tm, tn;
+            coords(t, tm, tn);
+            const uint32_t buf = lt & 1, m = tm * 256 + rank * 128 + quad * 32 + lane;
+            const float ra = m < p.g.M && p.g.a_rows ? p.g.a_rows[m] : 1.f;
+            if (!wait(acc_full(buf), (lt >> 1) & 1, abortp, 5)) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + buf * C::kSecond + ((uint32_t)(quad * 32) << 16);
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t ch = (2 * i + half + (buf ? 0 : 6)) & 7, n = tn * bn + ch * 32;
+                uint32_t v[32];
+                if (ch * 32 < bn) {
+                    __syncwarp();
+                    tmem_ld32(acc + ch * 32, v);
+                    tmem_ld_wait();
+                }
+                if (i == 0 || i == 3) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) arrive_at(in_cta(i == 0 ? shared_free : acc_empty(buf), 0));
+                }
+                if (ch * 32 < bn && m < p.g.M && n < p.g.N) store32<T>(p.g, v, m, n, ra, vec);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_barrier();   // the partner is done with this CTA's shared memory and TMEM
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// ---- few tokens: weights as the 128-row operand ---------------------------------------------------------------
+struct SwapArgs {
+    GemmArgs g;
+    uint32_t nt, splits;     // tokens per tile (a multiple of 16; 128 where there are several tiles); CTAs that share a tile's K
+    uint32_t tmem_cols;
+    uint32_t stages;
+};
+
+template <int FMT>
+struct Swap {
+    static constexpr int kTiles = kBK / (4 * (int)block_of(FMT));
+    static constexpr int kScale = kTiles * kTileBytes;
+    static constexpr int kThreads = 32 * 6;
+    static constexpr int kMaxStages = 8;
+    static __host__ __device__ uint32_t stage_bytes(uint32_t nt) { return 128 * 128 + nt * 128; }   // multiples of 1024
+};
+
+template <int FMT, class T>
+__global__ void __launch_bounds__(Swap<FMT>::kThreads)
+fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_sa,
+                const __grid_constant__ CUtensorMap map_sw, const SwapArgs p) {
+    using C = Swap<FMT>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int abort_flag;
+    __shared__ __align__(8) uint64_t bars[2 * C::kMaxStages + 2];
+    const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u, stage = C::stage_bytes(p.nt), scales0 = base + p.stages * stage;
+    float *part = reinterpret_cast<float *>(smem_raw + (base - smem_u32(smem_raw)));   // [token][128 channels], over the stages
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](uint32_t s) { return bar0 + 8u * s; };
+    auto empty = [&](uint32_t s) { return bar0 + 8u * (C::kMaxStages + s); };
+    const uint32_t acc_full = bar0 + 8u * 2 * C::kMaxStages, drained = acc_full + 8;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = p.splits > 1 ? ctarank() : 0;
+    const uint32_t tn = blockIdx.x / p.splits, t0 = blockIdx.y * p.nt;
+    const uint32_t ktiles = (p.g.K + kBK - 1) / kBK, k0 = rank * ktiles / p.splits, k1 = (rank + 1) * ktiles / p.splits;
+
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        for (uint32_t s = 0; s < p.stages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        mbar_init(acc_full, 1);
+        mbar_init(drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot, sfa = tmem + p.nt, sfb = sfa + 4 * C::kTiles;   // columns behind the accumulator
+    volatile int *abortp = &abort_flag;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            bool ok = true;
+            const uint32_t bytes = stage + 2 * C::kScale;
+            auto weights = [&](uint32_t k, uint32_t s) {
+                mbar_expect_tx(full(s), bytes);
+                load_2d<1>(base + s * stage, &map_w, full(s), k * 128, tn * 128);
+                load_3d<1>(scales0 + s * 2 * C::kScale, &map_sw, full(s), 0, k * C::kTiles, tn);
+            };
+            auto tokens = [&](uint32_t k, uint32_t s) {
+                load_2d<1>(base + s * stage + 128 * 128, &map_a, full(s), k * 128, t0);
+                load_3d<1>(scales0 + s * 2 * C::kScale + C::kScale, &map_sa, full(s), 0, k * C::kTiles, t0 >> 7);
+            };
+            // the first round of stages: weights at once, tokens when the launch in front (their quantizer) is done
+            const uint32_t head = min(p.stages, k1 - k0);
+            for (uint32_t i = 0; i < head; ++i) weights(k0 + i, i);
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (uint32_t i = 0; i < head; ++i) tokens(k0 + i, i);
+            for (uint32_t i = head; i < k1 - k0; ++i) {
+                const uint32_t s = i % p.stages, ph = (i / p.stages) & 1;
+                if (!(ok = wait(empty(s), ph ^ 1, abortp, 11))) break;
+                weights(k0 + i, s);
+                tokens(k0 + i, s);
+            }
+            if (!ok) leave_copies_behind();
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            bool ok = true, issued = false;
+            for (uint32_t i = 0; i < k1 - k0; ++i) {
+                const uint32_t s = i % p.stages, ph = (i / p.stages) & 1;
+                if (!(ok = wait(full(s), ph, abortp, 12))) break;
+                tc_fence_after();
+                const uint32_t sa = base + s * stage, sc = scales0 + s * 2 * C::kScale;
+                issue_stage<FMT, 1>(tmem, sa, sa + 128 * 128, sc, sc + C::kScale, sfa, sfb, 1, 128, p.nt, i == 0);
+                issued = true;
+                commit<1>(empty(s));
+            }
+            if (ok) commit<1>(acc_full);
+            else if (issued) {
+                commit<1>(drained);
+                const uint64_t b0 = globaltimer();
+                while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
+            }
+        }
+    } else {
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (wait(acc_full, 0, abortp, 13)) {
+            tc_fence_after();
+            const uint32_t quad = warp & 3, acc = tmem + ((quad * 32) << 16);
+            for (uint32_t c = 0; c < p.nt; c += 16) {
+                uint32_t v[16];
+                __syncwarp();
+                tmem_ld16(acc + c, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) part[(c + j) * 128 + quad * 32 + lane] = __uint_as_float(v[j]);
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (p.splits > 1) cluster_barrier();
+    // The partial sums of the cluster's CTAs meet in distributed shared memory; each CTA adds and stores a share of the
+    // outputs, four channels of one token per thread and step, always in the order of the CTAs.
+    if (!abort_flag) {
+        const uint32_t tokens = min(p.nt, p.g.M - t0), units = tokens * 32;
+        uint16_t *out = reinterpret_cast<uint16_t *>(p.g.out);
+        const uint16_t *bias = reinterpret_cast<const uint16_t *>(p.g.bias);
+        const bool vec = (p.g.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
+        for (uint32_t u = rank * C::kThreads + threadIdx.x; u < units; u += p.splits * C::kThreads) {
+            const uint32_t t = u >> 5, c = (u & 31) * 4, n = tn * 128 + c, m = t0 + t;
+            if (n >= p.g.N) continue;
+            float y[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint32_t local = smem_u32(part + t * 128 + c);
+            for (uint32_t s = 0; s < p.splits; ++s) {
+                float4 f;
+                if (p.splits > 1)
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(in_cta(local, s)));
+                else
+                    f = *reinterpret_cast<const float4 *>(part + t * 128 + c);
+                y[0] += f.x; y[1] += f.y; y[2] += f.z; y[3] += f.w;
+            }
+            const float ra = p.g.a_rows ? p.g.a_rows[m] : 1.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < p.g.N) y[j] = finish(y[j], ra, p.g.w_rows ? __ldg(p.g.w_rows + n + j) : 1.f, bias ? Two<T>::up1(__ldg(bias + n + j)) : 0.f);
+            uint16_t *o = out + (size_t)m * p.g.ldo + n;
+            const uint2 w = make_uint2(Two<T>::down(y[0], y[1]), Two<T>::down(y[2], y[3]));
+            if (vec && n + 4 <= p.g.N) {
+                *reinterpret_cast<uint2 *>(o) = w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (n + j < p.g.N) o[j] = (uint16_t)((j < 2 ? w.x : w.y) >> (16 * (j & 1)));
+            }
+        }
+    }
+    if (p.splits > 1) cluster_barrier();   // the others have read this CTA's partial sums
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, p.tmem_cols);
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                              const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeFn encoder() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+        return ok ? (EncodeFn)p : (EncodeFn) nullptr;
+    }();
+    return fn;
+}
+// Codes [rows, K/2] in boxes of 128 bytes x box_rows, 128-byte swizzle. A new descriptor per call: nothing is kept.
+static int map_codes(CUtensorMap *m, const uint8_t *p, uint32_t rows, uint32_t K, uint32_t box_rows) {
+    const EncodeFn f = encoder();
+    if (!f) return DUQ4_ERR_DEVICE;
+    const cuuint64_t dims[2] = {K / 2, rows}, strides[1] = {K / 2};
+    const cuuint32_t box[2] = {128, box_rows}, one[2] = {1, 1};
+    return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? DUQ4_OK : DUQ4_ERR_SHAPE;
+}
+// Block scales as [blocks of 128 rows][tiles of a row][512 bytes]; tiles beyond the row's end read as zero.
+static int map_scales(CUtensorMap *m, const uint8_t *p, int format, uint32_t rows, uint32_t K, uint32_t box_blocks) {
+    const EncodeFn f = encoder();
+    if (!f) return DUQ4_ERR_DEVICE;
+    const uint32_t tiles = scale_tiles(format, K), per_stage = kBK / (4 * block_of(format));
+    const cuuint64_t dims[3] = {kTileBytes / 4, tiles, cdiv(rows, 128)}, strides[2] = {kTileBytes, (cuuint64_t)tiles * kTileBytes};
+    const cuuint32_t box[3] = {kTileBytes / 4, per_stage, box_blocks}, one[3] = {1, 1, 1};
+    return f(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t *>(p), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? DUQ4_OK : DUQ4_ERR_SHAPE;
+}
+
+template <class F>
+static int launch(F *kernel, uint32_t gx, uint32_t gy, uint32_t threads, uint32_t smem, uint32_t cluster, bool overlap, cudaStream_t st, const CUtensorMap (&maps)[4],
+                  const void *args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(gx, gy);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = overlap ? 2 : 1;
+    void *a[] = {(void *)&maps[0], (void *)&maps[1], (void *)&maps[2], (void *)&maps[3], const_cast<void *>(args)};
+    const cudaError_t e = cudaLaunchKernelExC(&cfg, (const void *)kernel, a);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return (int)e;
+    }
     return launch_status();
+}
+
+template <int FMT, class T>
+static int launch_pair(const GemmArgs &g, cudaStream_t st) {
+    using C = Pair<FMT>;
+    static DeviceOnce once;
+    const int dev = current_device_slot();
+    if (dev < 0) return DUQ4_ERR_DEVICE;
+    int rc = once.run(dev, [] { return (int)cudaFuncSetAttribute(fp4_pair_kernel<FMT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
+    if (rc) return rc;
+    const uint32_t pairs = (uint32_t)sm_count_current_device() / 2;
+    PairArgs p{g, cdiv(g.M, 256), 0, 256};
+    if ((uint64_t)p.tiles_m * cdiv(g.N, 256) * 2 <= pairs) p.bn = 128;
+    p.tiles_n = cdiv(g.N, p.bn);
+    CUtensorMap maps[4];
+    if ((rc = map_codes(&maps[0], g.a, g.M, g.K, 128)) || (rc = map_codes(&maps[1], g.w, g.N, g.K, p.bn / 2)) ||
+        (rc = map_scales(&maps[2], g.a_scales, FMT, g.M, g.K, 1)) || (rc = map_scales(&maps[3], g.w_scales, FMT, g.N, g.K, p.bn / 128)))
+        return rc;
+    if ((uint64_t)p.tiles_m * p.tiles_n > 0x7FFFFFFFull) return DUQ4_ERR_SHAPE;
+    const uint32_t n = p.tiles_m * p.tiles_n < pairs ? p.tiles_m * p.tiles_n : pairs;
+    return launch(fp4_pair_kernel<FMT, T>, 2 * n, 1, C::kThreads, C::kSmem, 2, false, st, maps, &p);
+}
+
+template <int FMT, class T>
+static int launch_swap(const GemmArgs &g, cudaStream_t st, bool overlap) {
+    using C = Swap<FMT>;
+    constexpr uint32_t kMaxSmem = 232448 - 1024;
+    static DeviceOnce once;
+    const int dev = current_device_slot();
+    if (dev < 0) return DUQ4_ERR_DEVICE;
+    int rc = once.run(dev, [] { return (int)cudaFuncSetAttribute(fp4_swap_kernel<FMT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem); });
+    if (rc) return rc;
+    SwapArgs p{g, 0, 1, 0, 0};
+    p.nt = g.M > 128 ? 128 : (g.M + 15) / 16 * 16;
+    const uint32_t tiles_n = cdiv(g.N, 128), tiles_m = cdiv(g.M, p.nt), ktiles = cdiv(g.K, (uint32_t)kBK);
+    const uint32_t cols = p.nt + 8 * C::kTiles;
+    p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
+    const uint32_t per_stage = C::stage_bytes(p.nt) + 2 * C::kScale;
+    // two CTAs per SM: about 110 KiB of stages each
+    p.stages = (113 * 1024 - 1024) / per_stage;
+    if (p.stages > (uint32_t)C::kMaxStages) p.stages = C::kMaxStages;
+    // K over up to eight CTAs of a cluster until the GPU is full
+    const uint32_t slots = 2 * (uint32_t)sm_count_current_device();
+    while (p.splits < 8 && tiles_n * tiles_m * p.splits * 2 <= slots && ktiles >= p.splits * 2) p.splits *= 2;
+    uint32_t smem = p.stages * per_stage;
+    if (smem < p.nt * 512u) smem = p.nt * 512u;
+    smem += 1024;
+    if (tiles_m > 65535) return DUQ4_ERR_SHAPE;
+    CUtensorMap maps[4];
+    if ((rc = map_codes(&maps[0], g.a, g.M, g.K, p.nt)) || (rc = map_codes(&maps[1], g.w, g.N, g.K, 128)) ||
+        (rc = map_scales(&maps[2], g.a_scales, FMT, g.M, g.K, 1)) || (rc = map_scales(&maps[3], g.w_scales, FMT, g.N, g.K, 1)))
+        return rc;
+    return launch(fp4_swap_kernel<FMT, T>, tiles_n * p.splits, tiles_m, C::kThreads, smem, p.splits, overlap, st, maps, &p);
+}
+
+template <int FMT, class T>
+static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
+    return a.M <= 128 ? launch_swap<FMT, T>(a, st, overlap) : launch_pair<FMT, T>(a, st);
 }
 
 static int check_gemm(int format, int dtype, uint32_t N, uint32_t K, uint64_t ldo) {
@@ -88,14 +638,27 @@ static int check_gemm(int format, int dtype, uint32_t N, uint32_t K, uint64_t ld
 }
 static bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-static int run(int format, int dtype, const GemmArgs &a, cudaStream_t st) {
-    if (format == kMX) return dtype == DUQ4_DTYPE_F16 ? gemm<kMX, __half>(a, st) : gemm<kMX, __nv_bfloat16>(a, st);
-    return dtype == DUQ4_DTYPE_F16 ? gemm<kNV, __half>(a, st) : gemm<kNV, __nv_bfloat16>(a, st);
+static int run(int format, int dtype, const GemmArgs &a, cudaStream_t st, bool overlap) {
+    if (format == kMX) return dtype == DUQ4_DTYPE_F16 ? gemm<kMX, __half>(a, st, overlap) : gemm<kMX, __nv_bfloat16>(a, st, overlap);
+    return dtype == DUQ4_DTYPE_F16 ? gemm<kNV, __half>(a, st, overlap) : gemm<kNV, __nv_bfloat16>(a, st, overlap);
 }
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
 }  // namespace fp4
+
+int fp4_status_read(int32_t *out) {
+    int v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, g_fp4_status, sizeof(int));
+    if (e != cudaSuccess) return (int)e;
+    *out = v;
+    if (v != 0) {
+        int zero = 0;
+        cudaMemcpyToSymbol(g_fp4_status, &zero, sizeof(int));
+    }
+    return DUQ4_OK;
+}
+
 }  // namespace duq4
 
 using namespace duq4;
@@ -116,7 +679,7 @@ int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales,
         !aligned(W_row_scales, 4) || !aligned(bias, 2) || !aligned(out, 2))
         return DUQ4_ERR_ALIGN;
     const GemmArgs a{M, N, K, A, A_block_scales, W, W_block_scales, A_row_scales, W_row_scales, bias, out, ldo};
-    return run(format, dtype, a, (cudaStream_t)stream);
+    return run(format, dtype, a, (cudaStream_t)stream, false);
 }
 
 size_t duq4_linear_fp4_workspace_bytes(int format, uint32_t M, uint32_t K) {
@@ -133,11 +696,15 @@ int duq4_linear_fp4_from_16bit(int format, int dtype, const void *x, const uint8
     if (M == 0 || N == 0) return DUQ4_OK;
     if (!x || !W || !W_block_scales || !out) return DUQ4_ERR_NULL;
     if (!workspace || !aligned(workspace, 256) || workspace_bytes < duq4_linear_fp4_workspace_bytes(format, M, K)) return DUQ4_ERR_WORKSPACE;
+    if (!aligned(W, 16) || !aligned(W_block_scales, 16) || !aligned(W_row_scales, 4) || !aligned(bias, 2) || !aligned(out, 2)) return DUQ4_ERR_ALIGN;
     uint8_t *codes = (uint8_t *)workspace, *scales = codes + up256((size_t)M * (K / 2));
     float *rows = format == kNV ? (float *)(scales + up256(duq4_fp4_scale_bytes(format, M, K))) : nullptr;
     rc = duq4_fp4_quantize(format, dtype, x, M, K, K, codes, scales, rows, stream);
     if (rc) return rc;
-    return duq4_linear_fp4(format, codes, scales, rows, W, W_block_scales, W_row_scales, M, N, K, bias, dtype, out, ldo, stream);
+    const GemmArgs a{M, N, K, codes, scales, W, W_block_scales, rows, W_row_scales, bias, out, ldo};
+    // The product may start while the quantizer runs: the quantizer is an ordinary launch, so everything that was queued
+    // before it (the weights' upload among it) is done when it starts; what it writes itself is waited for in the kernel.
+    return run(format, dtype, a, (cudaStream_t)stream, true);
 }
 
 }  // extern "C"

@@ -140,6 +140,8 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
     __shared__ float sm_f[NT / 32][4];
     const uint32_t chunks = a.cols >> 4;
     const int lane = threadIdx.x & 31;
+    // a product launched behind the quantizer may start and fetch its weights (nothing happens without such a launch)
+    if (SRC == SRC_PLAIN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         Chunk d[CH];
         const uint16_t *xr = a.x + (size_t)row * a.ldx;
