@@ -46,11 +46,12 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
     return mbar_wait(bar, parity, abort_flag, &g_fp4_status, code);
 }
 
-// Instruction descriptor of the block-scaled kinds: e2m1 x e2m1 -> f32, both operands K-major. `sf`: which bytes of the
-// 32-bit scale words the instruction takes (0 or 2; two scales per instruction of the 32-blocks, four of the 16-blocks).
+// Instruction descriptor of the block-scaled kinds: e2m1 x e2m1 -> f32, both operands K-major. (Bits 4-5 and 29-30 name the
+// bytes of the 32-bit scale words that an instruction takes: 0 or 2; two scales per instruction of the 32-blocks, four of
+// the 16-blocks.)
 template <int FMT>
-__device__ __forceinline__ uint32_t block_idesc(int m, uint32_t n, uint32_t sf) {
-    return (sf << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((FMT == kMX ? 1u : 0u) << 23) | ((uint32_t)(m >> 4) << 24) | (sf << 29);
+__device__ __forceinline__ uint32_t block_idesc(int m, uint32_t n) {
+    return (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((FMT == kMX ? 1u : 0u) << 23) | ((uint32_t)(m >> 4) << 24);
 }
 // Scale tile in shared memory for tcgen05.cp: 8 rows of 16 bytes are contiguous, groups of 8 rows 128 bytes apart.
 __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
@@ -74,26 +75,30 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32
 }
 #undef DUQ4_FP4_MMA
 
+// One thread of a warp that runs converged: the operands of what it issues then stay in uniform registers. A stage takes
+// up to 18 issues; with the loop on one lane alone each took about 50 ns (4096 x 8192 x 28672, nvfp4: 0.83 ms).
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
 // One stage: its scale tiles to TMEM, its four MMAs. Scale tiles lie [block of 128 rows][tile] in shared memory and
-// [tile][block of rows] in TMEM (four columns each), so that the rows of one MMA are contiguous. a_blocks, b_blocks:
-// 128-row blocks of either operand in this CTA's shared memory.
-template <int FMT, int CG>
-__device__ __forceinline__ void issue_stage(uint32_t d, uint32_t sa, uint32_t sb, uint32_t ssa, uint32_t ssb, uint32_t ta, uint32_t tb,
-                                            uint32_t b_blocks, int m, uint32_t n, bool first) {
+// [tile][block of rows] in TMEM (four columns each), so that the rows of one MMA are contiguous. BB: 128-row blocks of B.
+template <int FMT, int CG, int BB>
+__device__ __forceinline__ void issue_stage(uint32_t d, uint64_t da, uint64_t db, uint64_t dsa, uint64_t dsb, uint32_t ta, uint32_t tb, uint32_t idesc0,
+                                            bool first) {
     constexpr int kTiles = kBK / (4 * (int)block_of(FMT));   // 2 or 4 scale tiles per stage and block of rows
 #pragma unroll
-    for (int j = 0; j < kTiles; ++j) copy_scales<CG>(ta + j * 4, scale_desc(ssa + j * kTileBytes));
+    for (int j = 0; j < kTiles; ++j) copy_scales<CG>(ta + j * 4, dsa + j * (kTileBytes >> 4));
 #pragma unroll
     for (int j = 0; j < kTiles; ++j)
-        for (uint32_t b = 0; b < b_blocks; ++b)
-            copy_scales<CG>(tb + (j * b_blocks + b) * 4, scale_desc(ssb + (b * kTiles + j) * kTileBytes));
-    const uint64_t da = make_desc(sa), db = make_desc(sb);
+#pragma unroll
+        for (int b = 0; b < BB; ++b) copy_scales<CG>(tb + (j * BB + b) * 4, dsb + (b * kTiles + j) * (kTileBytes >> 4));
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
         const int j = FMT == kMX ? kk >> 1 : kk;
         const uint32_t sf = FMT == kMX ? (kk & 1) * 2 : 0;
-        mma<FMT, CG>(d, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), block_idesc<FMT>(m, n, sf), ta + j * 4, tb + j * b_blocks * 4,
-                     !first || kk > 0);
+        mma<FMT, CG>(d, da + (uint64_t)(kk * 2), db + (uint64_t)(kk * 2), idesc0 | (sf << 4) | (sf << 29), ta + j * 4, tb + j * BB * 4, !first || kk > 0);
     }
 }
 
@@ -220,7 +225,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     auto acc_empty = [&](int b) { return bar0 + 8u * (2 * C::kStages + 2 + b); };   // the leader's: epilogue warps of both
     const uint32_t shared_free = bar0 + 8u * (2 * C::kStages + 4);           // the leader's: the shared columns are read
     const uint32_t drained = bar0 + 8u * (2 * C::kStages + 5);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const uint32_t rank = ctarank(), pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
     const uint32_t tiles = p.tiles_m * p.tiles_n, ksteps = (p.g.K + kBK - 1) / kBK, bn = p.bn;
 
@@ -279,32 +284,41 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (!ok) leave_copies_behind();
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             uint32_t it = 0, lt = 0;
             bool ok = true, issued = false;
+            const bool wide = bn == 256;
+            const uint32_t idesc = block_idesc<FMT>(256, bn);
+            const uint64_t desc_a = make_desc(base), desc_s = scale_desc(scales0);
             for (uint32_t t = pair; ok && t < tiles; t += npairs, ++lt) {
                 const uint32_t buf = lt & 1;
                 if (!(ok = wait(acc_empty(buf), ((lt >> 1) & 1) ^ 1, abortp, 2))) break;
                 if (lt > 0 && !(ok = wait(shared_free, (lt - 1) & 1, abortp, 3))) break;
                 tc_fence_after();
+                const uint32_t d = tmem + buf * C::kSecond;
                 for (uint32_t ks = 0; ks < ksteps; ++ks, ++it) {
                     const uint32_t s = it % C::kStages, ph = (it / C::kStages) & 1;
                     if (!(ok = wait(full(s), ph, abortp, 4))) break;
                     tc_fence_after();
-                    const uint32_t sa = base + s * 2 * C::kOperand, sc = scales0 + s * C::kScaleStage;
-                    issue_stage<FMT, 2>(tmem + buf * C::kSecond, sa, sa + C::kOperand, sc, sc + C::kScaleA, tmem + C::kSfa, tmem + C::kSfb, bn / 128,
-                                        256, bn, ks == 0);
+                    const uint64_t da = desc_a + s * (2 * C::kOperand >> 4), ds = desc_s + s * (C::kScaleStage >> 4);
+                    if (elected()) {
+                        if (wide)
+                            issue_stage<FMT, 2, 2>(d, da, da + (C::kOperand >> 4), ds, ds + (C::kScaleA >> 4), tmem + C::kSfa, tmem + C::kSfb, idesc, ks == 0);
+                        else
+                            issue_stage<FMT, 2, 1>(d, da, da + (C::kOperand >> 4), ds, ds + (C::kScaleA >> 4), tmem + C::kSfa, tmem + C::kSfb, idesc, ks == 0);
+                        commit<2>(empty(s));
+                        commit<2>(in_cta(empty(s), 1));
+                        if (ks + 1 == ksteps) {
+                            commit<2>(acc_full(buf));
+                            commit<2>(in_cta(acc_full(buf), 1));
+                        }
+                    }
+                    __syncwarp();
                     issued = true;
-                    commit<2>(empty(s));
-                    commit<2>(in_cta(empty(s), 1));
-                }
-                if (ok) {
-                    commit<2>(acc_full(buf));
-                    commit<2>(in_cta(acc_full(buf), 1));
                 }
             }
             if (!ok && issued) {
-                commit<2>(drained);
+                if (elected()) commit<2>(drained);
                 const uint64_t t0 = globaltimer();
                 while (!mbar_try(drained, 0) && globaltimer() - t0 < kPtxWaitLimitNs) __nanosleep(1000);
             }
@@ -384,7 +398,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     auto full = [&](uint32_t s) { return bar0 + 8u * s; };
     auto empty = [&](uint32_t s) { return bar0 + 8u * (C::kMaxStages + s); };
     const uint32_t acc_full = bar0 + 8u * 2 * C::kMaxStages, drained = acc_full + 8;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
     const uint32_t rank = p.splits > 1 ? ctarank() : 0;
     const uint32_t tn = blockIdx.x / p.splits, t0 = blockIdx.y * p.nt;
     const uint32_t ktiles = (p.g.K + kBK - 1) / kBK, k0 = rank * ktiles / p.splits, k1 = (rank + 1) * ktiles / p.splits;
@@ -436,23 +450,26 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             if (!ok) leave_copies_behind();
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            bool ok = true, issued = false;
-            for (uint32_t i = 0; i < k1 - k0; ++i) {
-                const uint32_t s = i % p.stages, ph = (i / p.stages) & 1;
-                if (!(ok = wait(full(s), ph, abortp, 12))) break;
-                tc_fence_after();
-                const uint32_t sa = base + s * stage, sc = scales0 + s * 2 * C::kScale;
-                issue_stage<FMT, 1>(tmem, sa, sa + 128 * 128, sc, sc + C::kScale, sfa, sfb, 1, 128, p.nt, i == 0);
-                issued = true;
+        bool ok = true, issued = false;
+        const uint32_t idesc = block_idesc<FMT>(128, p.nt);
+        const uint64_t desc_w = make_desc(base), desc_s = scale_desc(scales0);
+        for (uint32_t i = 0; i < k1 - k0; ++i) {
+            const uint32_t s = i % p.stages, ph = (i / p.stages) & 1;
+            if (!(ok = wait(full(s), ph, abortp, 12))) break;
+            tc_fence_after();
+            const uint64_t dw = desc_w + s * (stage >> 4), ds = desc_s + s * (2 * C::kScale >> 4);
+            if (elected()) {
+                issue_stage<FMT, 1, 1>(tmem, dw, dw + (128 * 128 >> 4), ds, ds + (C::kScale >> 4), sfa, sfb, idesc, i == 0);
                 commit<1>(empty(s));
+                if (i + 1 == k1 - k0) commit<1>(acc_full);
             }
-            if (ok) commit<1>(acc_full);
-            else if (issued) {
-                commit<1>(drained);
-                const uint64_t b0 = globaltimer();
-                while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
-            }
+            __syncwarp();
+            issued = true;
+        }
+        if (!ok && issued) {
+            if (elected()) commit<1>(drained);
+            const uint64_t b0 = globaltimer();
+            while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
         }
     } else {
         asm volatile("griddepcontrol.wait;" ::: "memory");
