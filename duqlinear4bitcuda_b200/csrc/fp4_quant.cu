@@ -22,124 +22,178 @@ struct RowArgs {
     uint16_t *residual_out;
     uint32_t gate_per_row;
     float residual_scale;
-    double eps;
+    double eps, inv_cols;         // 1 / cols
     float clip;
     // results
     uint8_t *codes;               // OUT_ROW: the 16-bit row itself
     uint8_t *block_scales;        // OUT_SYM / OUT_ASYM: fp16 scales [rows]
     void *row_scales;             // OUT_NV: float [rows]; OUT_ASYM: fp16 zero-points [rows]
+    uint32_t wide;                // every 16-bit tensor and row starts on a 32-byte boundary
 };
 
 struct Chunk {                    // 16 neighbours of a row
     uint32_t w[8];
 };
-__device__ __forceinline__ Chunk load_chunk(const uint16_t *p) {
+// Plain (not read-only-path) accesses: the norm's tensors may be written in place.
+__device__ __forceinline__ Chunk load_chunk(const uint16_t *p, bool wide) {
     Chunk c;
-    const uint4 a = __ldg(reinterpret_cast<const uint4 *>(p)), b = __ldg(reinterpret_cast<const uint4 *>(p) + 1);
-    c.w[0] = a.x; c.w[1] = a.y; c.w[2] = a.z; c.w[3] = a.w;
-    c.w[4] = b.x; c.w[5] = b.y; c.w[6] = b.z; c.w[7] = b.w;
+    if (wide) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(c.w[0]), "=r"(c.w[1]), "=r"(c.w[2]), "=r"(c.w[3]), "=r"(c.w[4]), "=r"(c.w[5]), "=r"(c.w[6]), "=r"(c.w[7])
+                     : "l"(p));
+    } else {
+        const uint4 a = reinterpret_cast<const uint4 *>(p)[0], b = reinterpret_cast<const uint4 *>(p)[1];
+        c.w[0] = a.x; c.w[1] = a.y; c.w[2] = a.z; c.w[3] = a.w;
+        c.w[4] = b.x; c.w[5] = b.y; c.w[6] = b.z; c.w[7] = b.w;
+    }
     return c;
 }
-// The same without the read-only path, for tensors that the call may write in place.
-__device__ __forceinline__ Chunk load_chunk_rw(const uint16_t *p) {
-    Chunk c;
-    const uint4 a = reinterpret_cast<const uint4 *>(p)[0], b = reinterpret_cast<const uint4 *>(p)[1];
-    c.w[0] = a.x; c.w[1] = a.y; c.w[2] = a.z; c.w[3] = a.w;
-    c.w[4] = b.x; c.w[5] = b.y; c.w[6] = b.z; c.w[7] = b.w;
-    return c;
+__device__ __forceinline__ void store_chunk(uint16_t *p, const Chunk &c, bool wide) {
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(c.w[0]), "r"(c.w[1]), "r"(c.w[2]), "r"(c.w[3]),
+                     "r"(c.w[4]), "r"(c.w[5]), "r"(c.w[6]), "r"(c.w[7]) : "memory");
+    } else {
+        reinterpret_cast<uint4 *>(p)[0] = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]);
+        reinterpret_cast<uint4 *>(p)[1] = make_uint4(c.w[4], c.w[5], c.w[6], c.w[7]);
+    }
 }
-__device__ __forceinline__ void store_chunk(uint16_t *p, const Chunk &c) {
-    reinterpret_cast<uint4 *>(p)[0] = make_uint4(c.w[0], c.w[1], c.w[2], c.w[3]);
-    reinterpret_cast<uint4 *>(p)[1] = make_uint4(c.w[4], c.w[5], c.w[6], c.w[7]);
+
+// Two floats per instruction, each rounded as by itself.
+struct Pair2 {
+    uint64_t v;
+};
+__device__ __forceinline__ Pair2 pair2(float2 f) {
+    Pair2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(f.x), "f"(f.y));
+    return r;
+}
+__device__ __forceinline__ Pair2 both(float f) { return pair2(make_float2(f, f)); }
+__device__ __forceinline__ float2 unpair(Pair2 p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair2 add2(Pair2 a, Pair2 b) {
+    Pair2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair2 mul2(Pair2 a, Pair2 b) {
+    Pair2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Pair2 fma2(Pair2 a, Pair2 b, Pair2 c) {
+    Pair2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+// -x / d for two quotients: by minus the approximate reciprocal of d, then one step of iterative refinement,
+// q + (x + q d) ninv with q = -x / d nearly. The residual is exact (fma), so what is left of the reciprocal's error is its
+// square, and the result is the nearest float wherever q and d are normal numbers. (The negated quotient, because then a
+// zero keeps its sign without an instruction for it.)
+__device__ __forceinline__ Pair2 minus_quotient2(Pair2 x, Pair2 d, Pair2 ninv) {
+    const Pair2 q = mul2(x, ninv);
+    return fma2(fma2(q, d, x), ninv, q);
 }
 
 // h = silu(g) * u with the roundings of F.silu(gate) * up on 16-bit tensors: silu in 32 bits, rounded, then the product.
 template <class T>
 __device__ __forceinline__ uint32_t silu_mul_two(uint32_t g, uint32_t u) {
     const float2 x = Two<T>::up(g), y = Two<T>::up(u);
-    const float2 s = Two<T>::up(Two<T>::down(__fdiv_rn(x.x, 1.0f + expf(-x.x)), __fdiv_rn(x.y, 1.0f + expf(-x.y))));
-    return Two<T>::down(__fmul_rn(s.x, y.x), __fmul_rn(s.y, y.y));
+    float2 s;
+    const float2 d = make_float2(1.0f + expf(-x.x), 1.0f + expf(-x.y));
+    if (fmaxf(fabsf(x.x), fabsf(x.y)) < 80.f)   // d below 6e34 (a NaN beside a number passes and stays one)
+        s = unpair(minus_quotient2(pair2(x), pair2(d), pair2(make_float2(rcp_approx_ftz(-d.x), rcp_approx_ftz(-d.y)))));
+    else
+        s = make_float2(-__fdiv_rn(x.x, d.x), -__fdiv_rn(x.y, d.y));
+    s = unpair(mul2(pair2(Two<T>::up(Two<T>::down(s.x, s.y))), pair2(y)));
+    return Two<T>::down(s.x, s.y) ^ 0x80008000u;
 }
 
-// Sums over the block; every thread gets the result. `sm` must not be in use by an earlier reduction's readers.
-template <int NT>
+// Sums and maxima over the block; every thread gets the result. `sm` must not be in use by an earlier reduction's readers.
 __device__ __forceinline__ double block_sum(double v, double *sm) {
+    const uint32_t lane = threadIdx.x & 31, warps = blockDim.x >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+    if (warps == 1) return v;
+    if (lane == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
-    double r = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) r += sm[w];
-    return r;
+    v = lane < warps ? sm[lane] : 0.0;
+    for (uint32_t o = warps > 16 ? 16 : warps > 8 ? 8 : warps > 4 ? 4 : 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
 }
-template <int NT>
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *sm) {
+    const uint32_t lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     v = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
+    if (warps == 1) return v;
+    if (lane == 0) sm[threadIdx.x >> 5] = v;
     __syncthreads();
-    uint32_t r = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) r = max(r, sm[w]);
-    return r;
-}
-
-// 1 / sqrt(mean of squares + eps) of the row that the block's threads hold. Codes jump at borders and the layer behind
-// must not depend on the order of a sum, so the sum is carried with its rounding errors: squares of 16-bit values are
-// exact in 32 bits, and each addition's error is recovered (Knuth's two-sum) and summed beside. Only rows whose
-// squares leave the range of 32 bits (bfloat16 beyond 1e19, infinities) are summed again in 64 bits.
-template <class T, int NT, int CH>
-__device__ __forceinline__ float row_rstd(const Chunk (&d)[CH], uint32_t chunks, uint32_t cols, double eps, double *sm) {
-    float s = 0.f, c = 0.f;
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-        if (threadIdx.x + i * NT < chunks) {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float2 x = Two<T>::up(d[i].w[k]);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float p = __fmul_rn(h ? x.y : x.x, h ? x.y : x.x);
-                    const float t = __fadd_rn(s, p), b = __fsub_rn(t, s);
-                    c = __fadd_rn(c, __fadd_rn(__fsub_rn(s, __fsub_rn(t, b)), __fsub_rn(p, b)));
-                    s = t;
-                }
-            }
-        }
-    double sum = block_sum<NT>((double)s + (double)c, sm);
-    if (!(sum > 1e-24 && sum < 1e38)) {   // the same for every thread
-        double v = 0;
-#pragma unroll
-        for (int i = 0; i < CH; ++i)
-            if (threadIdx.x + i * NT < chunks) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const float2 x = Two<T>::up(d[i].w[k]);
-                    v += (double)x.x * x.x + (double)x.y * x.y;
-                }
-            }
-        __syncthreads();
-        sum = block_sum<NT>(v, sm);
-    }
-    return (float)(1.0 / sqrt(sum / cols + eps));
+    return __reduce_max_sync(0xffffffffu, lane < warps ? sm[lane] : 0u);
 }
 
 template <class T>
 __device__ __forceinline__ uint32_t chunk_top(const Chunk &c) {   // largest magnitude's bits (above kInf: a NaN)
-    uint32_t m = 0;
+    uint32_t m = Two<T>::abs_max(c.w[0], c.w[1]);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) m = __vmaxu2(m, c.w[k] & 0x7FFF7FFFu);
+    for (int k = 2; k < 8; ++k) m = Two<T>::abs_max(m, c.w[k]);
     return max(m & 0xFFFFu, m >> 16);
 }
 
-// One CTA of NT threads per row, CH chunks per thread.
-template <int SRC, class T, int OUT, int NT, int CH>
-__global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
-    __shared__ double sm_d[2][NT / 32];
-    __shared__ uint32_t sm_u[NT / 32];
-    __shared__ float sm_f[NT / 32][4];
-    const uint32_t chunks = a.cols >> 4;
+// 1 / sqrt(mean of squares + eps) of the row that the block's threads hold. Codes jump at borders and must not depend on
+// the order of a sum, so the sum is carried with its rounding errors. Squares of 16-bit values are exact in 32 bits; a
+// thread's sum S starts at a power of two beyond its largest square, so that in S' = S + x^2 the part that S takes,
+// S' - S, is exact and so is the rest, x^2 - (S' - S), which is summed beside it (Dekker's fast two-sum): four
+// operations a value, and an error of the square of a rounding. The threads' sums meet in 64 bits. Rows whose squares
+// leave the range of 32 bits (bfloat16 beyond 1e18 or below 1e-15, infinities, NaNs) are summed in 64 bits instead.
+// `again`: where the thread finds its row once more for that.
+template <class T, int CH>
+__device__ __forceinline__ float row_rstd(const Chunk (&d)[CH], const RowArgs &a, const uint16_t *again, double *sm) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < CH; ++i) top = max(top, chunk_top<T>(d[i]));
+    const float m = Two<T>::up1(top), m2 = m * m;
+    const float start = __uint_as_float((__float_as_uint(m2) & 0x7F800000u) + 0x01000000u);   // in (2 m^2, 4 m^2]
+    const bool odd = top != 0 && !(m2 > 1e-30f && m2 < 1e36f);
+    const Pair2 minus_one = both(-1.f);
+    Pair2 s = both(start), c = both(0.f);
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {   // chunks beyond the row's end hold zeros
+            const Pair2 x = pair2(Two<T>::up(d[i].w[k]));
+            const Pair2 t = fma2(x, x, s);
+            c = add2(c, fma2(x, x, fma2(t, minus_one, s)));
+            s = t;
+        }
+    const float2 sf = unpair(s), cf = unpair(c);
+    double sum = ((double)(sf.x - start) + (double)(sf.y - start)) + ((double)cf.x + (double)cf.y);   // sf - start is exact
+    if (odd) {
+        sum = 0;
+#pragma unroll 1
+        for (uint32_t c = threadIdx.x; c < a.cols >> 4; c += blockDim.x)
+#pragma unroll 1
+            for (int k = 0; k < 8; ++k) {
+                const float2 x = Two<T>::up(reinterpret_cast<const volatile uint32_t *>(again + c * 16)[k]);
+                sum += (double)x.x * x.x + (double)x.y * x.y;
+            }
+    }
+    const double v = block_sum(sum, sm) * a.inv_cols + a.eps;
+    if (!(v > 1e-30 && v < 1e30)) return (float)(1.0 / sqrt(v));
+    // one Newton step in 64 bits from the 32-bit root: relative error about 1e-14
+    const double r = (double)rsqrtf((float)v);
+    return (float)(r + r * (0.5 - 0.5 * v * r * r));
+}
+
+// One CTA per row, CH chunks per thread.
+template <int SRC, class T, int OUT, int CH>
+__global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
+    __shared__ double sm_d[2][32];
+    __shared__ uint32_t sm_u[32];
+    __shared__ float sm_f[32][4];
+    const uint32_t chunks = a.cols >> 4, NT = blockDim.x;
     const int lane = threadIdx.x & 31;
+    const bool wide = a.wide != 0;
     // a product launched behind the quantizer may start and fetch its weights (nothing happens without such a launch)
     if (SRC == SRC_PLAIN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -149,9 +203,9 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
         for (int i = 0; i < CH; ++i) {
             const uint32_t c = threadIdx.x + i * NT;
             if (c < chunks) {
-                d[i] = SRC == SRC_NORM ? load_chunk_rw(xr + c * 16) : load_chunk(xr + c * 16);
+                d[i] = load_chunk(xr + c * 16, wide);
                 if (SRC == SRC_SILU) {
-                    const Chunk u = load_chunk(xr + a.up_offset + c * 16);
+                    const Chunk u = load_chunk(xr + a.up_offset + c * 16, wide);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) d[i].w[k] = silu_mul_two<T>(d[i].w[k], u.w[k]);
                 }
@@ -164,45 +218,44 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
             const size_t base = (size_t)row * a.cols;
             if (a.residual) {
                 float rstd = 1.f;
-                if (a.post_weight) rstd = row_rstd<T, NT, CH>(d, chunks, a.cols, a.eps, sm_d[0]);
+                if (a.post_weight) rstd = row_rstd<T, CH>(d, a, xr, sm_d[0]);
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
                     const uint32_t c = threadIdx.x + i * NT;
                     if (c >= chunks) continue;
-                    const Chunk r = load_chunk_rw(a.residual + base + c * 16);
-                    Chunk pw, g;
-                    if (a.post_weight) pw = load_chunk(a.post_weight + c * 16);
-                    if (a.gate) g = load_chunk(a.gate + (a.gate_per_row ? base : 0) + c * 16);
+                    const Chunk r = load_chunk(a.residual + base + c * 16, wide);
+                    Pair2 y[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] = pair2(Two<T>::up(d[i].w[k]));
+                    if (a.post_weight) {
+                        const Chunk w = load_chunk(a.post_weight + c * 16, wide);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) y[k] = mul2(mul2(y[k], both(rstd)), pair2(Two<T>::up(w.w[k])));
+                    }
+                    if (a.gate) {
+                        const Chunk w = load_chunk(a.gate + (a.gate_per_row ? base : 0) + c * 16, wide);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) y[k] = mul2(y[k], pair2(Two<T>::up(w.w[k])));
+                    }
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        float2 y = Two<T>::up(d[i].w[k]);
-                        const float2 rr = Two<T>::up(r.w[k]);
-                        if (a.post_weight) {
-                            const float2 w = Two<T>::up(pw.w[k]);
-                            y.x = __fmul_rn(__fmul_rn(y.x, rstd), w.x);
-                            y.y = __fmul_rn(__fmul_rn(y.y, rstd), w.y);
-                        }
-                        if (a.gate) {
-                            const float2 w = Two<T>::up(g.w[k]);
-                            y.x = __fmul_rn(y.x, w.x);
-                            y.y = __fmul_rn(y.y, w.y);
-                        }
-                        d[i].w[k] = Two<T>::down(__fadd_rn(rr.x, __fmul_rn(y.x, a.residual_scale)),
-                                                 __fadd_rn(rr.y, __fmul_rn(y.y, a.residual_scale)));
+                        // one by one: a two-float product and a two-float sum behind it are contracted into an fma
+                        const float2 yk = unpair(y[k]), rk = Two<T>::up(r.w[k]);
+                        d[i].w[k] = Two<T>::down(__fadd_rn(rk.x, __fmul_rn(yk.x, a.residual_scale)), __fadd_rn(rk.y, __fmul_rn(yk.y, a.residual_scale)));
                     }
-                    store_chunk(a.residual_out + base + c * 16, d[i]);
+                    store_chunk(a.residual_out + base + c * 16, d[i], wide);
                 }
             }
-            const float rstd = row_rstd<T, NT, CH>(d, chunks, a.cols, a.eps, sm_d[1]);
+            const float rstd = row_rstd<T, CH>(d, a, a.residual ? a.residual_out + base : xr, sm_d[1]);
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 const uint32_t c = threadIdx.x + i * NT;
                 if (c >= chunks) continue;
-                const Chunk w = load_chunk(a.weight + c * 16);
+                const Chunk w = load_chunk(a.weight + c * 16, wide);
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
-                    const float2 x = Two<T>::up(d[i].w[k]), ww = Two<T>::up(w.w[k]);
-                    d[i].w[k] = Two<T>::down(__fmul_rn(__fmul_rn(x.x, rstd), ww.x), __fmul_rn(__fmul_rn(x.y, rstd), ww.y));
+                    const float2 o = unpair(mul2(mul2(pair2(Two<T>::up(d[i].w[k])), both(rstd)), pair2(Two<T>::up(w.w[k]))));
+                    d[i].w[k] = Two<T>::down(o.x, o.y);
                 }
             }
         }
@@ -210,7 +263,7 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
                 const uint32_t c = threadIdx.x + i * NT;
-                if (c < chunks) store_chunk(reinterpret_cast<uint16_t *>(a.codes) + (size_t)row * a.cols + c * 16, d[i]);
+                if (c < chunks) store_chunk(reinterpret_cast<uint16_t *>(a.codes) + (size_t)row * a.cols + c * 16, d[i], wide);
             }
         } else if (OUT == OUT_SYM || OUT == OUT_ASYM) {
             // the framework's integer formats: statistics, scale and codes of quant_fused_vec_kernel on the row h
@@ -249,7 +302,7 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
         } else {
             constexpr int FMT = OUT == OUT_NV ? kNV : kMX;
             const uint32_t tiles = scale_tiles(FMT, a.cols);
-            float row_scale = 1.f;
+            float row_scale = 1.f, six = 6.f, inv6 = 0.f;
             if (FMT == kNV) {
                 uint32_t top = 0;   // over the blocks without infinities and NaNs
 #pragma unroll
@@ -257,11 +310,13 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
                     const uint32_t t = chunk_top<T>(d[i]);
                     if (t < Two<T>::kInf) top = max(top, t);
                 }
-                top = block_max<NT>(top, sm_u);
+                top = block_max(top, sm_u);
                 // 8 bits, so that 6 * row_scale and block scale * row_scale are exact
                 row_scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(Two<T>::up1(top), 2688.f)));
                 row_scale = fmaxf(row_scale, 7.703719777548943e-34f);   // 2^-110
                 if (threadIdx.x == 0) reinterpret_cast<float *>(a.row_scales)[row] = row_scale;
+                six = 6.f * row_scale;
+                inv6 = __fdiv_rn(1.f, six);
             }
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
@@ -275,32 +330,36 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
                     // 2^(floor(log2 top) - 2): the exponent field of the float, less 2
                     const int e = max((int)(__float_as_uint(Two<T>::up1(top)) >> 23) - 2, 0);
                     const float inv = special ? 0.f : __uint_as_float((uint32_t)(254 - e) << 23);
+                    const Pair2 inv2 = both(inv);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const float2 x = Two<T>::up(special ? 0u : d[i].w[k]);
-                        q[k >> 2][2 * (k & 3)] = __fmul_rn(x.x, inv);
-                        q[k >> 2][2 * (k & 3) + 1] = __fmul_rn(x.y, inv);
+                        const float2 y = unpair(mul2(pair2(Two<T>::up(d[i].w[k])), inv2));
+                        q[k >> 2][2 * (k & 3)] = y.x;
+                        q[k >> 2][2 * (k & 3) + 1] = y.y;
                     }
                     scale = special ? 0xFFu : (uint32_t)e;
                 } else {
-                    scale = special ? 0x7Fu : e4m3_of(__fdiv_rn(Two<T>::up1(top), 6.f * row_scale));
+                    // top / (6 row_scale): the middle of two e4m3 numbers exactly or at least 2^-15 away from it, so the
+                    // refined quotient rounds as the exact one
+                    const float t = Two<T>::up1(top), t0 = __fmul_rn(t, inv6);
+                    scale = special ? 0x7Fu : e4m3_of(__fmaf_rn(__fmaf_rn(-t0, six, t), inv6, t0));
                     const float dd = special ? 0.f : __fmul_rn(e4m3_to_float(scale), row_scale);
-                    const float inv = dd > 0.f ? __fdiv_rn(1.f, dd) : 0.f;
-                    // quotient by the reciprocal, then one step of refinement: a 16-bit value divided by the 12-bit dd is
-                    // the middle of two codes exactly or is at least 2^-15 away from it, so the code is that of x / dd
+                    const float inv = dd > 0.f ? rcp_approx_ftz(dd) : 0.f;
+                    // x / dd, a 16-bit value by a 12-bit one: as far from the middles of two codes
+                    const Pair2 dd2 = both(dd), ninv2 = both(-inv);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
-                        const float2 x = Two<T>::up(special ? 0u : d[i].w[k]);
-                        const float a0 = __fmul_rn(x.x, inv), a1 = __fmul_rn(x.y, inv);
-                        q[k >> 2][2 * (k & 3)] = __fmaf_rn(-__fmaf_rn(a0, dd, -x.x), inv, a0);   // (-0 stays -0)
-                        q[k >> 2][2 * (k & 3) + 1] = __fmaf_rn(-__fmaf_rn(a1, dd, -x.y), inv, a1);
+                        const float2 y = unpair(minus_quotient2(pair2(Two<T>::up(d[i].w[k])), dd2, ninv2));
+                        q[k >> 2][2 * (k & 3)] = y.x;
+                        q[k >> 2][2 * (k & 3) + 1] = y.y;
                     }
                 }
                 if (c >= chunks) scale = 0;   // padding blocks of the last scale tile
                 if (c < chunks) {
                     uint2 w;
-                    w.x = e2m1x8(q[0]);
-                    w.y = e2m1x8(q[1]);
+                    const uint32_t keep = special ? 0u : 0xFFFFFFFFu;   // (a bad block's quotients are NaNs)
+                    w.x = (e2m1x8(q[0]) ^ (FMT == kNV ? 0x88888888u : 0u)) & keep;
+                    w.y = (e2m1x8(q[1]) ^ (FMT == kNV ? 0x88888888u : 0u)) & keep;
                     *reinterpret_cast<uint2 *>(a.codes + (size_t)row * (a.cols >> 1) + c * 8) = w;
                 }
                 // four block scales are one word of a tile, stored by the first lane of the 8 (4) that hold them
@@ -319,7 +378,7 @@ __global__ void __launch_bounds__(NT) fp4_row_kernel(const RowArgs a) {
 template <int FMT, class T>
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
                                                           const float *__restrict__ row_scales, uint32_t rows, uint32_t cols,
-                                                          T *__restrict__ out) {
+                                                          T *__restrict__ out, bool wide) {
     const uint32_t chunks = cols >> 4, tiles = scale_tiles(FMT, cols);
     const uint64_t total = (uint64_t)rows * chunks;
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
@@ -342,7 +401,7 @@ __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t *__restr
             Chunk o;
 #pragma unroll
             for (int k = 0; k < 8; ++k) o.w[k] = Two<T>::down(v[2 * k], v[2 * k + 1]);
-            store_chunk(reinterpret_cast<uint16_t *>(out + i * 16), o);
+            store_chunk(reinterpret_cast<uint16_t *>(out + i * 16), o, wide);
         }
     }
 }
@@ -353,14 +412,21 @@ static bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintp
 constexpr uint32_t kMaxCols = 65536;
 
 template <int SRC, class T, int OUT>
-static int launch_rows(const RowArgs &a, cudaStream_t st) {
+static int launch_rows(RowArgs a, cudaStream_t st) {
     const uint32_t chunks = a.cols >> 4;
     const uint32_t grid = a.rows < 148u * 64u ? a.rows : 148u * 64u;
-    if (chunks <= 128) fp4_row_kernel<SRC, T, OUT, 128, 1><<<grid, 128, 0, st>>>(a);
-    else if (chunks <= 512) fp4_row_kernel<SRC, T, OUT, 256, 2><<<grid, 256, 0, st>>>(a);
-    else if (chunks <= 1024) fp4_row_kernel<SRC, T, OUT, 512, 2><<<grid, 512, 0, st>>>(a);
-    else if (chunks <= 2048) fp4_row_kernel<SRC, T, OUT, 1024, 2><<<grid, 1024, 0, st>>>(a);
-    else fp4_row_kernel<SRC, T, OUT, 1024, 4><<<grid, 1024, 0, st>>>(a);
+    a.inv_cols = 1.0 / a.cols;
+    uintptr_t bits = reinterpret_cast<uintptr_t>(a.x) | (uintptr_t)(a.ldx * 2) | (uintptr_t)a.up_offset * 2 | reinterpret_cast<uintptr_t>(a.residual) |
+                     reinterpret_cast<uintptr_t>(a.residual_out) | reinterpret_cast<uintptr_t>(a.post_weight) | reinterpret_cast<uintptr_t>(a.gate) |
+                     reinterpret_cast<uintptr_t>(a.weight);
+    if (OUT == OUT_ROW) bits |= reinterpret_cast<uintptr_t>(a.codes);
+    a.wide = (bits & 31) == 0;
+    auto threads = [&](uint32_t ch) { return cdiv(cdiv(chunks, ch), 32) * 32; };
+    // Few rows: 16 columns per thread, so that a row is done soonest (1 x 4096, norm: 2.4 us against 2.6 with 32). Many rows:
+    // 32, so that the reductions' fixed cost is spread (4096 x 8192, norm: 29 us against 38 with 16 and 33 with 64).
+    if (a.rows < 296 && chunks <= 1024) fp4_row_kernel<SRC, T, OUT, 1><<<grid, threads(1), 0, st>>>(a);
+    else if (chunks <= 2048) fp4_row_kernel<SRC, T, OUT, 2><<<grid, threads(2), 0, st>>>(a);
+    else fp4_row_kernel<SRC, T, OUT, 4><<<grid, threads(4), 0, st>>>(a);
     return launch_status();
 }
 
@@ -476,7 +542,7 @@ int duq4_fp4_dequantize(int format, int dtype, const uint8_t *codes, const uint8
     const uint64_t total = (uint64_t)rows * (cols >> 4);
     const uint32_t grid = (uint32_t)((total + 255) / 256 < 148u * 32u ? (total + 255) / 256 : 148u * 32u);
     auto go = [&](auto fmt, auto *o) {
-        fp4_dequant_kernel<decltype(fmt)::value><<<grid, 256, 0, st>>>(codes, block_scales, row_scales, rows, cols, o);
+        fp4_dequant_kernel<decltype(fmt)::value><<<grid, 256, 0, st>>>(codes, block_scales, row_scales, rows, cols, o, aligned(out, 32));
     };
     auto by_type = [&](auto fmt) {
         if (dtype == DUQ4_DTYPE_F16) go(fmt, (__half *)out);
