@@ -161,7 +161,8 @@ struct Pair {
     static constexpr int kStages = FMT == kMX ? 6 : 5;
     static constexpr int kOperand = 128 * 128;                 // one CTA's 128 rows of codes
     static constexpr int kScaleA = kTiles * kTileBytes, kScaleStage = 3 * kScaleA;   // own tokens, then all channels of the tile
-    static constexpr int kSmem = 1024 + kStages * (2 * kOperand + kScaleStage);
+    static constexpr int kStore = 1024;                        // an epilogue warp's 32 rows x 16 channels
+    static constexpr int kSmem = 1024 + kStages * (2 * kOperand + kScaleStage) + 8 * kStore;
     static constexpr int kThreads = 32 * 10;
     // TMEM: two accumulators of 256 columns and the scales do not fit in 512 columns side by side, so the second
     // accumulator starts inside the first: its first 64 columns are the first one's last 64. The epilogue takes those
@@ -170,42 +171,85 @@ struct Pair {
     static_assert(kSfb + 8 * kTiles <= 512 && kSmem <= 232448 - 512, "does not fit");
 };
 
-// 32 neighbouring channels of one token from the accumulator to memory.
+// Channel factors and bias of 8 neighbouring channels, all inside N.
 template <class T>
-__device__ __forceinline__ void store32(const GemmArgs &a, const uint32_t (&v)[32], uint32_t m, uint32_t n, float ra, bool vec) {
-    uint16_t *row = reinterpret_cast<uint16_t *>(a.out) + (size_t)m * a.ldo + n;
-    const uint16_t *bias = reinterpret_cast<const uint16_t *>(a.bias);
-    if (vec && n + 32 <= a.N) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float y[8];
-            if (a.w_rows) {
-                const float4 s0 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n + q * 8)), s1 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n + q * 8) + 1);
-                const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = s[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = 1.f;
-            }
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (bias) b = __ldg(reinterpret_cast<const uint4 *>(bias + n + q * 8));
-            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
-            uint32_t o[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float2 bf = Two<T>::up(bw[j]);
-                o[j] = Two<T>::down(finish(__uint_as_float(v[q * 8 + 2 * j]), ra, y[2 * j], bf.x),
-                                    finish(__uint_as_float(v[q * 8 + 2 * j + 1]), ra, y[2 * j + 1], bf.y));
-            }
-            reinterpret_cast<uint4 *>(row)[q] = make_uint4(o[0], o[1], o[2], o[3]);
-        }
+__device__ __forceinline__ void channel_terms(const GemmArgs &a, uint32_t n, float (&f)[8], float (&b)[8]) {
+    if (a.w_rows) {
+        const float4 s0 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n)), s1 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n) + 1);
+        f[0] = s0.x; f[1] = s0.y; f[2] = s0.z; f[3] = s0.w; f[4] = s1.x; f[5] = s1.y; f[6] = s1.z; f[7] = s1.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (n + j < a.N)
-                row[j] = (uint16_t)(Two<T>::down(finish(__uint_as_float(v[j]), ra, a.w_rows ? a.w_rows[n + j] : 1.f,
-                                                        bias ? Two<T>::up1(bias[n + j]) : 0.f), 0.f) & 0xFFFFu);
+        for (int j = 0; j < 8; ++j) f[j] = 1.f;
+    }
+    uint4 w = make_uint4(0, 0, 0, 0);
+    if (a.bias) w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.bias) + n));
+    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 p = Two<T>::up(ww[j]);
+        b[2 * j] = p.x;
+        b[2 * j + 1] = p.y;
+    }
+}
+// A warp's 32 tokens (one per lane) x 32 neighbouring channels from the accumulator to memory. vec: the channel vectors
+// are 16-byte aligned; how: rows of the result start on 32 (2) or 16 (1) bytes or neither (0). `stage`: the warp's 1 KiB.
+template <class T>
+__device__ __forceinline__ void store32(const GemmArgs &a, const uint32_t (&v)[32], uint32_t m0, uint32_t n, float ra, bool vec, int how, uint8_t *stage) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t m = m0 + lane;
+    const uint16_t *bias = reinterpret_cast<const uint16_t *>(a.bias);
+    const bool inside = n + 32 <= a.N;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t o[8];
+        if (vec && inside) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                float f[8], b[8];
+                channel_terms<T>(a, n + h * 16 + q * 8, f, b);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = h * 16 + q * 8 + 2 * j;
+                    o[q * 4 + j] = Two<T>::down(finish(__uint_as_float(v[e]), ra, f[2 * j], b[2 * j]),
+                                                finish(__uint_as_float(v[e + 1]), ra, f[2 * j + 1], b[2 * j + 1]));
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float y[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t c = min(n + h * 16 + 2 * j + e, a.N - 1);
+                    y[e] = finish(__uint_as_float(v[h * 16 + 2 * j + e]), ra, a.w_rows ? __ldg(a.w_rows + c) : 1.f, bias ? Two<T>::up1(__ldg(bias + c)) : 0.f);
+                }
+                o[j] = Two<T>::down(y[0], y[1]);
+            }
+        }
+        uint16_t *out = reinterpret_cast<uint16_t *>(a.out);
+        if (how && inside) {
+            uint16_t *row = out + (size_t)m * a.ldo + n + h * 16;
+            if (m < a.M) {
+                if (how == 2) {
+                    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]),
+                                 "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+                } else {
+                    reinterpret_cast<uint4 *>(row)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                    reinterpret_cast<uint4 *>(row)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+                }
+            }
+        } else {
+            // rows of any alignment: through shared memory, so that neighbouring lanes store neighbouring channels
+            // (stored lane by lane, 32 segments per instruction, a tile of 256 x 256 took longer than its MMAs)
+            reinterpret_cast<uint4 *>(stage + lane * 32)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+            reinterpret_cast<uint4 *>(stage + lane * 32)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            __syncwarp();
+            const uint32_t c = n + h * 16 + (lane & 15);
+#pragma unroll 4
+            for (int r = lane >> 4; r < 32; r += 2)
+                if (m0 + r < a.M && c < a.N) out[(size_t)(m0 + r) * a.ldo + c] = reinterpret_cast<const uint16_t *>(stage)[r * 16 + (lane & 15)];
+            __syncwarp();
+        }
     }
 }
 
@@ -327,13 +371,15 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         // Epilogue, eight warps: two per TMEM lane quadrant, which take the tile's 32-column chunks in turn, the shared
         // ones (6, 7 of the first accumulator, 0, 1 of the second) first.
         const int quad = warp & 3, half = (warp - 2) >> 2;
-        const bool vec = (p.g.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(p.g.out) & 15) == 0 &&
-                         (reinterpret_cast<uintptr_t>(p.g.w_rows) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.g.bias) & 15) == 0;
+        const bool vec = (reinterpret_cast<uintptr_t>(p.g.w_rows) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.g.bias) & 15) == 0;
+        const uintptr_t rows = reinterpret_cast<uintptr_t>(p.g.out) | (uintptr_t)(p.g.ldo * 2);
+        const int how = (rows & 31) == 0 ? 2 : (rows & 15) == 0 ? 1 : 0;
+        uint8_t *stage = smem_raw + (scales0 + C::kStages * C::kScaleStage - smem_u32(smem_raw)) + (warp - 2) * C::kStore;
         uint32_t lt = 0;
         for (uint32_t t = pair; t < tiles; t += npairs, ++lt) {
             uint32_t tm, tn;
             coords(t, tm, tn);
-            const uint32_t buf = lt & 1, m = tm * 256 + rank * 128 + quad * 32 + lane;
+            const uint32_t buf = lt & 1, m0 = tm * 256 + rank * 128 + quad * 32, m = m0 + lane;
             const float ra = m < p.g.M && p.g.a_rows ? p.g.a_rows[m] : 1.f;
             if (!wait(acc_full(buf), (lt >> 1) & 1, abortp, 5)) break;
             tc_fence_after();
@@ -352,7 +398,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     __syncwarp();
                     if (lane == 0) arrive_at(in_cta(i == 0 ? shared_free : acc_empty(buf), 0));
                 }
-                if (ch * 32 < bn && m < p.g.M && n < p.g.N) store32<T>(p.g, v, m, n, ra, vec);
+                if (ch * 32 < bn && m0 < p.g.M && n < p.g.N) store32<T>(p.g, v, m0, n, ra, vec, how, stage);
             }
         }
     }
@@ -644,6 +690,11 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, bool overlap) {
 
 template <int FMT, class T>
 static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
+#ifdef FORCE_PAIR
+    return launch_pair<FMT, T>(a, st);
+#elif defined(FORCE_SWAP)
+    return launch_swap<FMT, T>(a, st, overlap);
+#endif
     return a.M <= 128 ? launch_swap<FMT, T>(a, st, overlap) : launch_pair<FMT, T>(a, st);
 }
 
