@@ -418,6 +418,7 @@ struct SwapArgs {
     uint32_t nt, splits;     // tokens per tile (a multiple of 16; 128 where there are several tiles); CTAs that share a tile's K
     uint32_t tmem_cols;
     uint32_t stages;
+    uint32_t early;          // 1: the tokens' quantizer is the launch in front and may still run
 };
 
 template <int FMT>
@@ -425,7 +426,7 @@ struct Swap {
     static constexpr int kTiles = kBK / (4 * (int)block_of(FMT));
     static constexpr int kScale = kTiles * kTileBytes;
     static constexpr int kThreads = 32 * 6;
-    static constexpr int kMaxStages = 8;
+    static constexpr int kMaxStages = 10;
     static __host__ __device__ uint32_t stage_bytes(uint32_t nt) { return 128 * 128 + nt * 128; }   // multiples of 1024
 };
 
@@ -449,6 +450,16 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t tn = blockIdx.x / p.splits, t0 = blockIdx.y * p.nt;
     const uint32_t ktiles = (p.g.K + kBK - 1) / kBK, k0 = rank * ktiles / p.splits, k1 = (rank + 1) * ktiles / p.splits;
 
+    const uint32_t head = min(p.stages, k1 - k0);   // the first round of stages
+    auto weights = [&](uint32_t k, uint32_t s) {    // a stage's weights, and the bytes it waits for
+        mbar_expect_tx(full(s), stage + 2 * C::kScale);
+        load_2d<1>(base + s * stage, &map_w, full(s), k * 128, tn * 128);
+        load_3d<1>(scales0 + s * 2 * C::kScale, &map_sw, full(s), 0, k * C::kTiles, tn);
+    };
+    auto tokens = [&](uint32_t k, uint32_t s) {
+        load_2d<1>(base + s * stage + 128 * 128, &map_a, full(s), k * 128, t0);
+        load_3d<1>(scales0 + s * 2 * C::kScale + C::kScale, &map_sa, full(s), 0, k * C::kTiles, t0 >> 7);
+    };
     if (threadIdx.x == 0) {
         abort_flag = 0;
         for (uint32_t s = 0; s < p.stages; ++s) {
@@ -458,6 +469,10 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         mbar_init(acc_full, 1);
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (uint32_t i = 0; i < head; ++i) {   // before the CTA is set up
+            weights(k0 + i, i);
+            if (!p.early) tokens(k0 + i, i);
+        }
     }
     if (warp == 1) {
         tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
@@ -472,21 +487,10 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
-            const uint32_t bytes = stage + 2 * C::kScale;
-            auto weights = [&](uint32_t k, uint32_t s) {
-                mbar_expect_tx(full(s), bytes);
-                load_2d<1>(base + s * stage, &map_w, full(s), k * 128, tn * 128);
-                load_3d<1>(scales0 + s * 2 * C::kScale, &map_sw, full(s), 0, k * C::kTiles, tn);
-            };
-            auto tokens = [&](uint32_t k, uint32_t s) {
-                load_2d<1>(base + s * stage + 128 * 128, &map_a, full(s), k * 128, t0);
-                load_3d<1>(scales0 + s * 2 * C::kScale + C::kScale, &map_sa, full(s), 0, k * C::kTiles, t0 >> 7);
-            };
-            // the first round of stages: weights at once, tokens when the launch in front (their quantizer) is done
-            const uint32_t head = min(p.stages, k1 - k0);
-            for (uint32_t i = 0; i < head; ++i) weights(k0 + i, i);
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            for (uint32_t i = 0; i < head; ++i) tokens(k0 + i, i);
+            if (p.early) {
+                asm volatile("griddepcontrol.wait;" ::: "memory");
+                for (uint32_t i = 0; i < head; ++i) tokens(k0 + i, i);
+            }
             for (uint32_t i = head; i < k1 - k0; ++i) {
                 const uint32_t s = i % p.stages, ph = (i / p.stages) & 1;
                 if (!(ok = wait(empty(s), ph ^ 1, abortp, 11))) break;
@@ -518,50 +522,61 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
         }
     } else {
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        if (wait(acc_full, 0, abortp, 13)) {
-            tc_fence_after();
-            const uint32_t quad = warp & 3, acc = tmem + ((quad * 32) << 16);
-            for (uint32_t c = 0; c < p.nt; c += 16) {
-                uint32_t v[16];
-                __syncwarp();
-                tmem_ld16(acc + c, v);
-                tmem_ld_wait();
+        if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
+        wait(acc_full, 0, abortp, 13);
+        tc_fence_after();
+    }
+    if (warp >= 2 && !abort_flag) {
+        const uint32_t quad = warp & 3, acc = tmem + ((quad * 32) << 16);
+        for (uint32_t c = 0; c < p.nt; c += 16) {
+            uint32_t v[16];
+            __syncwarp();
+            tmem_ld16(acc + c, v);
+            tmem_ld_wait();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) part[(c + j) * 128 + quad * 32 + lane] = __uint_as_float(v[j]);
-            }
+            for (int j = 0; j < 16; ++j) part[(c + j) * 128 + quad * 32 + lane] = __uint_as_float(v[j]);
         }
         tc_fence_before();
     }
-    __syncthreads();
-    if (p.splits > 1) cluster_barrier();
     // The partial sums of the cluster's CTAs meet in distributed shared memory; each CTA adds and stores a share of the
-    // outputs, four channels of one token per thread and step, always in the order of the CTAs.
-    if (!abort_flag) {
-        const uint32_t tokens = min(p.nt, p.g.M - t0), units = tokens * 32;
-        uint16_t *out = reinterpret_cast<uint16_t *>(p.g.out);
-        const uint16_t *bias = reinterpret_cast<const uint16_t *>(p.g.bias);
-        const bool vec = (p.g.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0;
-        for (uint32_t u = rank * C::kThreads + threadIdx.x; u < units; u += p.splits * C::kThreads) {
-            const uint32_t t = u >> 5, c = (u & 31) * 4, n = tn * 128 + c, m = t0 + t;
-            if (n >= p.g.N) continue;
-            float y[4] = {0.f, 0.f, 0.f, 0.f};
-            const uint32_t local = smem_u32(part + t * 128 + c);
-            for (uint32_t s = 0; s < p.splits; ++s) {
-                float4 f;
-                if (p.splits > 1)
-                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(in_cta(local, s)));
-                else
-                    f = *reinterpret_cast<const float4 *>(part + t * 128 + c);
-                y[0] += f.x; y[1] += f.y; y[2] += f.z; y[3] += f.w;
-            }
-            const float ra = p.g.a_rows ? p.g.a_rows[m] : 1.f;
+    // tokens, a token per warp and step and four channels per thread, always in the order of the CTAs. (Sent to the storing
+    // CTA instead, 128 tokens, 4096 x 4096: 10.6 us against 9.4; 16 tokens: 6.8 against 7.2.)
+    const uint32_t tokens_here = min(p.nt, p.g.M - t0), c = (threadIdx.x & 31) * 4, n = tn * 128 + c;
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.g.out);
+    const uint16_t *bias = reinterpret_cast<const uint16_t *>(p.g.bias);
+    const bool vec = (p.g.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0 && n + 4 <= p.g.N;
+    float f[4], b[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (n + j < p.g.N) y[j] = finish(y[j], ra, p.g.w_rows ? __ldg(p.g.w_rows + n + j) : 1.f, bias ? Two<T>::up1(__ldg(bias + n + j)) : 0.f);
+    for (int j = 0; j < 4; ++j) {
+        const bool in = n + j < p.g.N;
+        f[j] = in && p.g.w_rows ? __ldg(p.g.w_rows + n + j) : 1.f;
+        b[j] = in && bias ? Two<T>::up1(__ldg(bias + n + j)) : 0.f;
+    }
+    if (p.splits > 1) cluster_barrier();
+    else __syncthreads();
+    if (!abort_flag && n < p.g.N) {
+        for (uint32_t t = rank * (C::kThreads / 32) + warp; t < tokens_here; t += p.splits * (C::kThreads / 32)) {
+            const uint32_t m = t0 + t, local = smem_u32(part + t * 128 + c);
+            const float ra = p.g.a_rows ? p.g.a_rows[m] : 1.f;
+            float4 y;
+            if (p.splits == 1) {
+                y = *reinterpret_cast<const float4 *>(part + t * 128 + c);
+            } else {
+                float4 v[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (s < p.splits)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w) : "r"(in_cta(local, s)));
+                y = v[0];
+#pragma unroll
+                for (int s = 1; s < 8; ++s)
+                    if (s < p.splits) { y.x += v[s].x; y.y += v[s].y; y.z += v[s].z; y.w += v[s].w; }
+            }
+            const uint2 w = make_uint2(Two<T>::down(finish(y.x, ra, f[0], b[0]), finish(y.y, ra, f[1], b[1])),
+                                       Two<T>::down(finish(y.z, ra, f[2], b[2]), finish(y.w, ra, f[3], b[3])));
             uint16_t *o = out + (size_t)m * p.g.ldo + n;
-            const uint2 w = make_uint2(Two<T>::down(y[0], y[1]), Two<T>::down(y[2], y[3]));
-            if (vec && n + 4 <= p.g.N) {
+            if (vec) {
                 *reinterpret_cast<uint2 *>(o) = w;
             } else {
 #pragma unroll
@@ -571,6 +586,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
     }
     if (p.splits > 1) cluster_barrier();   // the others have read this CTA's partial sums
+    else __syncthreads();
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -665,18 +681,24 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, bool overlap) {
     if (dev < 0) return DUQ4_ERR_DEVICE;
     int rc = once.run(dev, [] { return (int)cudaFuncSetAttribute(fp4_swap_kernel<FMT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem); });
     if (rc) return rc;
-    SwapArgs p{g, 0, 1, 0, 0};
+    SwapArgs p{g, 0, 1, 0, 0, overlap ? 1u : 0u};
     p.nt = g.M > 128 ? 128 : (g.M + 15) / 16 * 16;
     const uint32_t tiles_n = cdiv(g.N, 128), tiles_m = cdiv(g.M, p.nt), ktiles = cdiv(g.K, (uint32_t)kBK);
     const uint32_t cols = p.nt + 8 * C::kTiles;
     p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
     const uint32_t per_stage = C::stage_bytes(p.nt) + 2 * C::kScale;
-    // two CTAs per SM: about 110 KiB of stages each
-    p.stages = (113 * 1024 - 1024) / per_stage;
+    // K over up to eight CTAs of a cluster while there is an SM for each (M 16, 4096 x 4096: 9.0 / 8.3 / 7.5 / 7.6 us with 1 / 2 / 4 / 8;
+    // 22016 x 4096, 172 tiles: 13.1 / 17.5 us with 1 / 2, whose 344 CTAs do not fit at once)
+    const uint32_t sms = (uint32_t)sm_count_current_device();
+    while (p.splits < 8 && (uint64_t)tiles_n * tiles_m * p.splits * 2 <= sms && ktiles >= p.splits * 2) p.splits *= 2;
+#ifdef SPL
+    p.splits = SPL;
+#endif
+    // stages: an SM's shared memory for one CTA, or half of it (228 KiB, 1 KiB a CTA taken) for two
+    const bool alone = p.splits <= 2 && (uint64_t)tiles_n * tiles_m * p.splits <= sms;   // (wider clusters pack badly one CTA to an SM)
+    p.stages = ((alone ? 220 : 111) * 1024) / per_stage;
     if (p.stages > (uint32_t)C::kMaxStages) p.stages = C::kMaxStages;
-    // K over up to eight CTAs of a cluster until the GPU is full
-    const uint32_t slots = 2 * (uint32_t)sm_count_current_device();
-    while (p.splits < 8 && tiles_n * tiles_m * p.splits * 2 <= slots && ktiles >= p.splits * 2) p.splits *= 2;
+    if (p.stages > cdiv(ktiles, p.splits)) p.stages = cdiv(ktiles, p.splits);
     uint32_t smem = p.stages * per_stage;
     if (smem < p.nt * 512u) smem = p.nt * 512u;
     smem += 1024;
@@ -688,6 +710,11 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, bool overlap) {
     return launch(fp4_swap_kernel<FMT, T>, tiles_n * p.splits, tiles_m, C::kThreads, smem, p.splits, overlap, st, maps, &p);
 }
 
+// Which kernel. The pair kernel does a tile of 256 x 256 in about the time in which the other one does a tile of 128 x 128
+// (0.37 against 0.45 us for 256 columns of K, cold weights, all SMs at work), but it takes whole tiles of tokens and does not split K. Both
+// are priced by the columns of K that the busiest SM goes through (measured, nvfp4, pair / swap, us: 128 tokens x 22016 x 4096
+// 21.5 / 17.1; 256 x 22016 x 4096 21.5 / 29.1; 256 x 4096 x 11008 19.9 / 16.3; 512 x 4096 x 4096 11.7 / 14.2;
+// 4149 x 45 x 24800 36.7 / 16.8; 1024 x 1024 x 1024 7.8 / 9.0).
 template <int FMT, class T>
 static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
 #ifdef FORCE_PAIR
@@ -695,7 +722,14 @@ static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
 #elif defined(FORCE_SWAP)
     return launch_swap<FMT, T>(a, st, overlap);
 #endif
-    return a.M <= 128 ? launch_swap<FMT, T>(a, st, overlap) : launch_pair<FMT, T>(a, st);
+    if (a.M <= 128) return launch_swap<FMT, T>(a, st, overlap);
+    const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK);
+    const uint64_t pair_tiles = (uint64_t)cdiv(a.M, 256) * cdiv(a.N, 256), swap_tiles = (uint64_t)cdiv(a.M, 128) * cdiv(a.N, 128);
+    const uint64_t pair_cost = (pair_tiles + sms / 2 - 1) / (sms / 2) * ktiles * 37;
+    uint64_t splits = 1;
+    while (splits < 8 && swap_tiles * splits * 2 <= sms && ktiles >= splits * 2) splits *= 2;
+    const uint64_t swap_cost = (swap_tiles * splits + sms - 1) / sms * ((ktiles + splits - 1) / splits) * 45 + 200;
+    return swap_cost < pair_cost ? launch_swap<FMT, T>(a, st, overlap) : launch_pair<FMT, T>(a, st);
 }
 
 static int check_gemm(int format, int dtype, uint32_t N, uint32_t K, uint64_t ldo) {
