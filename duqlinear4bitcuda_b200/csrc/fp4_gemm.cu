@@ -161,8 +161,9 @@ struct Pair {
     static constexpr int kStages = FMT == kMX ? 6 : 5;
     static constexpr int kOperand = 128 * 128;                 // one CTA's 128 rows of codes
     static constexpr int kScaleA = kTiles * kTileBytes, kScaleStage = 3 * kScaleA;   // own tokens, then all channels of the tile
-    static constexpr int kStore = 1024;                        // an epilogue warp's 32 rows x 16 channels
-    static constexpr int kSmem = 1024 + kStages * (2 * kOperand + kScaleStage) + 8 * kStore;
+    static constexpr int kStore = 1024;                        // an epilogue warp's 32 rows x 16 channels,
+    static constexpr int kTerms = 128 * 6;                     // and the factors (float) and biases (16 bits) of its 128 channels
+    static constexpr int kSmem = 1024 + kStages * (2 * kOperand + kScaleStage) + 8 * (kStore + kTerms);
     static constexpr int kThreads = 32 * 10;
     // TMEM: two accumulators of 256 columns and the scales do not fit in 512 columns side by side, so the second
     // accumulator starts inside the first: its first 64 columns are the first one's last 64. The epilogue takes those
@@ -171,62 +172,28 @@ struct Pair {
     static_assert(kSfb + 8 * kTiles <= 512 && kSmem <= 232448 - 512, "does not fit");
 };
 
-// Channel factors and bias of 8 neighbouring channels, all inside N.
+// A warp's 32 tokens (one per lane) x 32 neighbouring channels from the accumulator to memory. f, bias: the channels'
+// factors and biases in shared memory; how: rows of the result start on 32 (2) or 16 (1) bytes or neither (0). `stage`: the
+// warp's 1 KiB.
 template <class T>
-__device__ __forceinline__ void channel_terms(const GemmArgs &a, uint32_t n, float (&f)[8], float (&b)[8]) {
-    if (a.w_rows) {
-        const float4 s0 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n)), s1 = __ldg(reinterpret_cast<const float4 *>(a.w_rows + n) + 1);
-        f[0] = s0.x; f[1] = s0.y; f[2] = s0.z; f[3] = s0.w; f[4] = s1.x; f[5] = s1.y; f[6] = s1.z; f[7] = s1.w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = 1.f;
-    }
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (a.bias) w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.bias) + n));
-    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 p = Two<T>::up(ww[j]);
-        b[2 * j] = p.x;
-        b[2 * j + 1] = p.y;
-    }
-}
-// A warp's 32 tokens (one per lane) x 32 neighbouring channels from the accumulator to memory. vec: the channel vectors
-// are 16-byte aligned; how: rows of the result start on 32 (2) or 16 (1) bytes or neither (0). `stage`: the warp's 1 KiB.
-template <class T>
-__device__ __forceinline__ void store32(const GemmArgs &a, const uint32_t (&v)[32], uint32_t m0, uint32_t n, float ra, bool vec, int how, uint8_t *stage) {
+__device__ __forceinline__ void store32(const GemmArgs &a, const uint32_t (&v)[32], uint32_t m0, uint32_t n, float ra, const float *f, const uint32_t *bias,
+                                        int how, uint8_t *stage) {
     const int lane = threadIdx.x & 31;
     const uint32_t m = m0 + lane;
-    const uint16_t *bias = reinterpret_cast<const uint16_t *>(a.bias);
     const bool inside = n + 32 <= a.N;
+    uint16_t *out = reinterpret_cast<uint16_t *>(a.out);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         uint32_t o[8];
-        if (vec && inside) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                float f[8], b[8];
-                channel_terms<T>(a, n + h * 16 + q * 8, f, b);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int e = h * 16 + q * 8 + 2 * j;
-                    o[q * 4 + j] = Two<T>::down(finish(__uint_as_float(v[e]), ra, f[2 * j], b[2 * j]),
-                                                finish(__uint_as_float(v[e + 1]), ra, f[2 * j + 1], b[2 * j + 1]));
-                }
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float y[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const uint32_t c = min(n + h * 16 + 2 * j + e, a.N - 1);
-                    y[e] = finish(__uint_as_float(v[h * 16 + 2 * j + e]), ra, a.w_rows ? __ldg(a.w_rows + c) : 1.f, bias ? Two<T>::up1(__ldg(bias + c)) : 0.f);
-                }
-                o[j] = Two<T>::down(y[0], y[1]);
-            }
+        for (int q = 0; q < 4; ++q) {
+            const float4 fq = *reinterpret_cast<const float4 *>(f + h * 16 + q * 4);
+            const uint2 bq = *reinterpret_cast<const uint2 *>(bias + h * 8 + q * 2);
+            const float2 b0 = Two<T>::up(bq.x), b1 = Two<T>::up(bq.y);
+            const int e = h * 16 + q * 4;
+            o[2 * q] = Two<T>::down(finish(__uint_as_float(v[e]), ra, fq.x, b0.x), finish(__uint_as_float(v[e + 1]), ra, fq.y, b0.y));
+            o[2 * q + 1] = Two<T>::down(finish(__uint_as_float(v[e + 2]), ra, fq.z, b1.x), finish(__uint_as_float(v[e + 3]), ra, fq.w, b1.y));
         }
-        uint16_t *out = reinterpret_cast<uint16_t *>(a.out);
         if (how && inside) {
             uint16_t *row = out + (size_t)m * a.ldo + n + h * 16;
             if (m < a.M) {
@@ -371,16 +338,27 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         // Epilogue, eight warps: two per TMEM lane quadrant, which take the tile's 32-column chunks in turn, the shared
         // ones (6, 7 of the first accumulator, 0, 1 of the second) first.
         const int quad = warp & 3, half = (warp - 2) >> 2;
-        const bool vec = (reinterpret_cast<uintptr_t>(p.g.w_rows) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.g.bias) & 15) == 0;
         const uintptr_t rows = reinterpret_cast<uintptr_t>(p.g.out) | (uintptr_t)(p.g.ldo * 2);
         const int how = (rows & 31) == 0 ? 2 : (rows & 15) == 0 ? 1 : 0;
-        uint8_t *stage = smem_raw + (scales0 + C::kStages * C::kScaleStage - smem_u32(smem_raw)) + (warp - 2) * C::kStore;
+        uint8_t *stage = smem_raw + (scales0 + C::kStages * C::kScaleStage - smem_u32(smem_raw)) + (warp - 2) * (C::kStore + C::kTerms);
+        float *factors = reinterpret_cast<float *>(stage + C::kStore);
+        uint16_t *biases = reinterpret_cast<uint16_t *>(factors + 128);
         uint32_t lt = 0;
         for (uint32_t t = pair; t < tiles; t += npairs, ++lt) {
             uint32_t tm, tn;
             coords(t, tm, tn);
             const uint32_t buf = lt & 1, m0 = tm * 256 + rank * 128 + quad * 32, m = m0 + lane;
             const float ra = m < p.g.M && p.g.a_rows ? p.g.a_rows[m] : 1.f;
+            // this warp's four chunks' channel terms, fetched while the tile is computed
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t n = tn * bn + ((2 * i + half + (buf ? 0 : 6)) & 7) * 32 + lane;
+                const bool in = n < p.g.N;
+                factors[i * 32 + lane] = in && p.g.w_rows ? p.g.w_rows[n] : 1.f;
+                biases[i * 32 + lane] = in && p.g.bias ? reinterpret_cast<const uint16_t *>(p.g.bias)[n] : (uint16_t)0;
+            }
+            __syncwarp();
             if (!wait(acc_full(buf), (lt >> 1) & 1, abortp, 5)) break;
             tc_fence_after();
             const uint32_t acc = tmem + buf * C::kSecond + ((uint32_t)(quad * 32) << 16);
@@ -398,7 +376,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     __syncwarp();
                     if (lane == 0) arrive_at(in_cta(i == 0 ? shared_free : acc_empty(buf), 0));
                 }
-                if (ch * 32 < bn && m0 < p.g.M && n < p.g.N) store32<T>(p.g, v, m0, n, ra, vec, how, stage);
+                if (ch * 32 < bn && m0 < p.g.M && n < p.g.N) store32<T>(p.g, v, m0, n, ra, factors + i * 32, reinterpret_cast<const uint32_t *>(biases + i * 32), how, stage);
             }
         }
     }
