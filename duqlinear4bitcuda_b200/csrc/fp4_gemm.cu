@@ -273,6 +273,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         tm = band * 16 + r % here;
     };
 
+    if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the rest of the columns, where a second launch does them
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
@@ -396,7 +397,7 @@ struct SwapArgs {
     uint32_t nt, splits;     // tokens per tile (a multiple of 16; 128 where there are several tiles); CTAs that share a tile's K
     uint32_t tmem_cols;
     uint32_t stages;
-    uint32_t early;          // 1: the tokens' quantizer is the launch in front and may still run
+    uint32_t early;          // the launch in front may still run: 1: it is the tokens' quantizer, 2: nothing is needed of it
 };
 
 template <int FMT>
@@ -449,7 +450,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (uint32_t i = 0; i < head; ++i) {   // before the CTA is set up
             weights(k0 + i, i);
-            if (!p.early) tokens(k0 + i, i);
+            if (p.early != 1) tokens(k0 + i, i);
         }
     }
     if (warp == 1) {
@@ -465,7 +466,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     if (warp == 0) {
         if (lane == 0) {
             bool ok = true;
-            if (p.early) {
+            if (p.early == 1) {
                 asm volatile("griddepcontrol.wait;" ::: "memory");
                 for (uint32_t i = 0; i < head; ++i) tokens(k0 + i, i);
             }
@@ -500,7 +501,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
         }
     } else {
-        if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");
         wait(acc_full, 0, abortp, 13);
         tc_fence_after();
     }
@@ -565,6 +566,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
     if (p.splits > 1) cluster_barrier();   // the others have read this CTA's partial sums
     else __syncthreads();
+    if (p.early == 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // this launch does not end before the one in front
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
@@ -650,8 +652,15 @@ static int launch_pair(const GemmArgs &g, cudaStream_t st) {
     return launch(fp4_pair_kernel<FMT, T>, 2 * n, 1, C::kThreads, C::kSmem, 2, false, st, maps, &p);
 }
 
+// CTAs that share a tile's K: up to eight while there is an SM for each (M 16, 4096 x 4096: 9.0 / 8.3 / 7.5 / 7.6 us with 1 / 2 / 4 /
+// 8; 22016 x 4096, 172 tiles: 13.1 / 17.5 us with 1 / 2, whose 344 CTAs do not fit at once).
+static uint32_t swap_splits(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
+    uint32_t splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= sms && ktiles >= splits * 2) splits *= 2;
+    return splits;
+}
 template <int FMT, class T>
-static int launch_swap(const GemmArgs &g, cudaStream_t st, bool overlap) {
+static int launch_swap(const GemmArgs &g, cudaStream_t st, uint32_t early) {
     using C = Swap<FMT>;
     constexpr uint32_t kMaxSmem = 232448 - 1024;
     static DeviceOnce once;
@@ -659,19 +668,14 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, bool overlap) {
     if (dev < 0) return DUQ4_ERR_DEVICE;
     int rc = once.run(dev, [] { return (int)cudaFuncSetAttribute(fp4_swap_kernel<FMT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem); });
     if (rc) return rc;
-    SwapArgs p{g, 0, 1, 0, 0, overlap ? 1u : 0u};
+    SwapArgs p{g, 0, 1, 0, 0, early};
     p.nt = g.M > 128 ? 128 : (g.M + 15) / 16 * 16;
     const uint32_t tiles_n = cdiv(g.N, 128), tiles_m = cdiv(g.M, p.nt), ktiles = cdiv(g.K, (uint32_t)kBK);
     const uint32_t cols = p.nt + 8 * C::kTiles;
     p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
     const uint32_t per_stage = C::stage_bytes(p.nt) + 2 * C::kScale;
-    // K over up to eight CTAs of a cluster while there is an SM for each (M 16, 4096 x 4096: 9.0 / 8.3 / 7.5 / 7.6 us with 1 / 2 / 4 / 8;
-    // 22016 x 4096, 172 tiles: 13.1 / 17.5 us with 1 / 2, whose 344 CTAs do not fit at once)
     const uint32_t sms = (uint32_t)sm_count_current_device();
-    while (p.splits < 8 && (uint64_t)tiles_n * tiles_m * p.splits * 2 <= sms && ktiles >= p.splits * 2) p.splits *= 2;
-#ifdef SPL
-    p.splits = SPL;
-#endif
+    p.splits = swap_splits((uint64_t)tiles_n * tiles_m, ktiles, sms);
     // stages: an SM's shared memory for one CTA, or half of it (228 KiB, 1 KiB a CTA taken) for two
     const bool alone = p.splits <= 2 && (uint64_t)tiles_n * tiles_m * p.splits <= sms;   // (wider clusters pack badly one CTA to an SM)
     p.stages = ((alone ? 220 : 111) * 1024) / per_stage;
@@ -685,14 +689,19 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, bool overlap) {
     if ((rc = map_codes(&maps[0], g.a, g.M, g.K, p.nt)) || (rc = map_codes(&maps[1], g.w, g.N, g.K, 128)) ||
         (rc = map_scales(&maps[2], g.a_scales, FMT, g.M, g.K, 1)) || (rc = map_scales(&maps[3], g.w_scales, FMT, g.N, g.K, 1)))
         return rc;
-    return launch(fp4_swap_kernel<FMT, T>, tiles_n * p.splits, tiles_m, C::kThreads, smem, p.splits, overlap, st, maps, &p);
+    return launch(fp4_swap_kernel<FMT, T>, tiles_n * p.splits, tiles_m, C::kThreads, smem, p.splits, early != 0, st, maps, &p);
 }
 
-// Which kernel. The pair kernel does a tile of 256 x 256 in about the time in which the other one does a tile of 128 x 128
-// (0.37 against 0.45 us for 256 columns of K, cold weights, all SMs at work), but it takes whole tiles of tokens and does not split K. Both
-// are priced by the columns of K that the busiest SM goes through (measured, nvfp4, pair / swap, us: 128 tokens x 22016 x 4096
-// 21.5 / 17.1; 256 x 22016 x 4096 21.5 / 29.1; 256 x 4096 x 11008 19.9 / 16.3; 512 x 4096 x 4096 11.7 / 14.2;
-// 4149 x 45 x 24800 36.7 / 16.8; 1024 x 1024 x 1024 7.8 / 9.0).
+// Which kernel. Both are priced in 10 ns by the columns of K that the busiest SM goes through, in steps of 256: 0.37 us for the
+// pair kernel's 256 x 256 (cold weights; a tile's epilogue hides behind the next tile), 0.45 us for the other one's
+// 128 x 128 with all SMs at work, and 2 us for its meeting. (Measured, nvfp4, pair / swap, us: 128 tokens x 22016 x 4096
+// 21.5 / 17.1; 256 x 22016 x 4096 21.5 / 29.1; 256 x 4096 x 11008 19.9 / 15.9; 512 x 4096 x 4096 11.0 / 13.8;
+// 4149 x 45 x 24800 36.7 / 16.8; 1024 x 1024 x 1024 6.8 / 8.7.)
+static uint64_t pair_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) { return (tiles + sms / 2 - 1) / (sms / 2) * ktiles * 37; }
+static uint64_t swap_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
+    const uint64_t splits = swap_splits(tiles, ktiles, sms);
+    return (tiles * splits + sms - 1) / sms * ((ktiles + splits - 1) / splits) * 45 + 200;
+}
 template <int FMT, class T>
 static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
 #ifdef FORCE_PAIR
@@ -701,13 +710,29 @@ static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
     return launch_swap<FMT, T>(a, st, overlap);
 #endif
     if (a.M <= 128) return launch_swap<FMT, T>(a, st, overlap);
-    const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK);
-    const uint64_t pair_tiles = (uint64_t)cdiv(a.M, 256) * cdiv(a.N, 256), swap_tiles = (uint64_t)cdiv(a.M, 128) * cdiv(a.N, 128);
-    const uint64_t pair_cost = (pair_tiles + sms / 2 - 1) / (sms / 2) * ktiles * 37;
-    uint64_t splits = 1;
-    while (splits < 8 && swap_tiles * splits * 2 <= sms && ktiles >= splits * 2) splits *= 2;
-    const uint64_t swap_cost = (swap_tiles * splits + sms - 1) / sms * ((ktiles + splits - 1) / splits) * 45 + 200;
-    return swap_cost < pair_cost ? launch_swap<FMT, T>(a, st, overlap) : launch_pair<FMT, T>(a, st);
+    const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK), tiles_m = cdiv(a.M, 256), tiles_n = cdiv(a.N, 256);
+    const uint64_t all = pair_price(tiles_m * tiles_n, ktiles, sms), blocks_m = cdiv(a.M, 128);
+    if (swap_price(blocks_m * cdiv(a.N, 128), ktiles, sms) < all) return launch_swap<FMT, T>(a, st, overlap);
+    // A last round that few tiles are left for: whole rounds by the pair kernel, the columns that are left by the other one,
+    // launched behind it (512 x 28672 x 8192, 3 rounds and 2 tiles of 256 x 256: 57.9 -> 53.3 us).
+    const uint64_t rest = tiles_m * tiles_n % (sms / 2), strip = rest ? (rest + tiles_m - 1) / tiles_m : 0;
+    if (strip && strip < tiles_n) {
+        const uint32_t n0 = (uint32_t)(tiles_n - strip) * 256;
+        const uint64_t both = pair_price(tiles_m * (tiles_n - strip), ktiles, sms) + swap_price(blocks_m * cdiv(a.N - n0, 128), ktiles, sms);
+        if (both < all) {
+            GemmArgs main = a, left = a;
+            main.N = n0;
+            left.N = a.N - n0;
+            left.w += (size_t)n0 * (a.K / 2);
+            left.w_scales += (size_t)(n0 / 128) * scale_tiles(FMT, a.K) * kTileBytes;
+            if (a.w_rows) left.w_rows += n0;
+            if (a.bias) left.bias = reinterpret_cast<const uint16_t *>(a.bias) + n0;
+            left.out = reinterpret_cast<uint16_t *>(a.out) + n0;
+            const int rc = launch_pair<FMT, T>(main, st);
+            return rc ? rc : launch_swap<FMT, T>(left, st, 2);
+        }
+    }
+    return launch_pair<FMT, T>(a, st);
 }
 
 static int check_gemm(int format, int dtype, uint32_t N, uint32_t K, uint64_t ldo) {

@@ -316,3 +316,22 @@ def _weights64(layer):
     byte = F.untile(layer.weight_scales.cpu().numpy(), rows, cols // F.BLOCK[layer.format])
     row = None if layer.weight_row_scales is None else layer.weight_row_scales.cpu().numpy()
     return F.values(layer.format, F.unpack(layer.weight.cpu().numpy()), byte, row)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(300, 9600, 4128), (600, 6500, 2080), (1000, 19001, 288)])
+def test_linear_whole_rounds_and_a_rest(fmt, dtype, m, n, k):
+    """Problems of more tiles than there are SM pairs, with columns left over behind whole rounds: rows and columns all over
+    the result against the definition, and a second call gives the same bits."""
+    ap, at, ar, av = F.random_operand(fmt, m, k, 1)
+    wp, wt, wr, wv = F.random_operand(fmt, n, k, 2)
+    if dtype == torch.float16:
+        wr, wv = wr * np.float32(2.0 ** -12), wv * 2.0 ** -12
+    args = [fmt, F.cuda(ap), F.cuda(at), F.cuda(ar), F.cuda(wp), F.cuda(wt), F.cuda(wr), None, dtype]
+    got = ops().linear_fp4(*args)
+    assert torch.equal(ops().linear_fp4(*args), got)
+    rows = sorted({0, 1, 127, 128, 255, 256, m // 2, m - 2, m - 1})
+    check_product(got[rows], av[rows], wv, None, dtype)
+    cols = sorted({0, 255, 256, n // 2, n - 513, n - 257, n - 256, n - 129, n - 1})
+    check_product(got[:, cols], av, wv[cols], None, dtype)
