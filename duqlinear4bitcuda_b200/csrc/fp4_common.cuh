@@ -68,10 +68,11 @@ struct Two<__half> {
     static constexpr uint32_t kInf = 0x7C00u;
     static __device__ __forceinline__ float2 up(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
     static __device__ __forceinline__ float up1(uint32_t bits) { return __half2float(__ushort_as_half((unsigned short)bits)); }
-    // larger magnitudes of two pairs, as bits without signs; a NaN wins
+    // larger magnitudes of two pairs, with signs of no meaning; a NaN wins
     static __device__ __forceinline__ uint32_t abs_max(uint32_t a, uint32_t b) {
-        const __half2 m = __hmax2_nan(__habs2(*reinterpret_cast<const __half2 *>(&a)), __habs2(*reinterpret_cast<const __half2 *>(&b)));
-        return *reinterpret_cast<const uint32_t *>(&m) & 0x7FFF7FFFu;
+        uint32_t r;
+        asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
     }
     static __device__ __forceinline__ uint32_t down(float a, float b) {
         const __half2 h = __floats2half2_rn(a, b);
@@ -86,8 +87,9 @@ struct Two<__nv_bfloat16> {
     }
     static __device__ __forceinline__ float up1(uint32_t bits) { return __uint_as_float(bits << 16); }
     static __device__ __forceinline__ uint32_t abs_max(uint32_t a, uint32_t b) {
-        const __nv_bfloat162 m = __hmax2_nan(__habs2(*reinterpret_cast<const __nv_bfloat162 *>(&a)), __habs2(*reinterpret_cast<const __nv_bfloat162 *>(&b)));
-        return *reinterpret_cast<const uint32_t *>(&m) & 0x7FFF7FFFu;
+        uint32_t r;
+        asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
     }
     static __device__ __forceinline__ uint32_t down(float a, float b) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);

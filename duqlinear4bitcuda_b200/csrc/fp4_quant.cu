@@ -137,6 +137,7 @@ __device__ __forceinline__ uint32_t chunk_top(const Chunk &c) {   // largest mag
     uint32_t m = Two<T>::abs_max(c.w[0], c.w[1]);
 #pragma unroll
     for (int k = 2; k < 8; ++k) m = Two<T>::abs_max(m, c.w[k]);
+    m &= 0x7FFF7FFFu;
     return max(m & 0xFFFFu, m >> 16);
 }
 
@@ -301,7 +302,8 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
             }
         } else {
             constexpr int FMT = OUT == OUT_NV ? kNV : kMX;
-            const uint32_t tiles = scale_tiles(FMT, a.cols);
+            uint8_t *codes = a.codes + (size_t)row * (a.cols >> 1);
+            uint8_t *scales = a.block_scales + scale_offset(scale_tiles(FMT, a.cols), row, 0);
             float row_scale = 1.f, six = 6.f, inv6 = 0.f;
             if (FMT == kNV) {
                 uint32_t top = 0;   // over the blocks without infinities and NaNs
@@ -360,14 +362,14 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
                     const uint32_t keep = special ? 0u : 0xFFFFFFFFu;   // (a bad block's quotients are NaNs)
                     w.x = (e2m1x8(q[0]) ^ (FMT == kNV ? 0x88888888u : 0u)) & keep;
                     w.y = (e2m1x8(q[1]) ^ (FMT == kNV ? 0x88888888u : 0u)) & keep;
-                    *reinterpret_cast<uint2 *>(a.codes + (size_t)row * (a.cols >> 1) + c * 8) = w;
+                    *reinterpret_cast<uint2 *>(codes + c * 8) = w;
                 }
                 // four block scales are one word of a tile, stored by the first lane of the 8 (4) that hold them
                 constexpr int kStep = FMT == kMX ? 2 : 1;
                 scale |= __shfl_down_sync(0xffffffffu, scale, kStep) << 8;
                 scale |= __shfl_down_sync(0xffffffffu, scale, 2 * kStep) << 16;
                 if ((lane & (4 * kStep - 1)) == 0 && c < chunks)
-                    *reinterpret_cast<uint32_t *>(a.block_scales + scale_offset(tiles, row, c / (4 * kStep))) = scale;
+                    *reinterpret_cast<uint32_t *>(scales + c / (4 * kStep) * 512) = scale;
             }
         }
         __syncthreads();   // the reductions' buffers are free for the next row
