@@ -425,9 +425,14 @@ static int launch_rows(RowArgs a, cudaStream_t st) {
     a.wide = (bits & 31) == 0;
     auto threads = [&](uint32_t ch) { return cdiv(cdiv(chunks, ch), 32) * 32; };
     // Few rows: 16 columns per thread, so that a row is done soonest (1 x 4096, norm: 2.4 us against 2.6 with 32). Many rows:
-    // 32, so that the reductions' fixed cost is spread (4096 x 8192, norm: 29 us against 38 with 16 and 33 with 64).
+    // 32, so that the reductions' fixed cost is spread (4096 x 8192, norm: 29 us against 38 with 16 and 33 with 64). Wide
+    // rows without a norm, whose registers allow it: 64, so that two rows fit an SM and one loads while the other computes
+    // (us with 32 / 64, nvfp4: 4096 x 8192 18.7 / 16.4, 2048 x 11008 17.1 / 13.5, 1024 x 28672 23.3 / 17.7, silu 2048 x 11008
+    // 35.8 / 31.5, 4096 x 8192 40.1 / 41.8; mxfp4: 2048 x 11008 10.8 / 10.7, silu 26.3 / 28.4, 2048 x 16384 15.9 / 13.9, silu
+    // 38.3 / 36.9; norm joint, 2048 x 16384: 55.3 / 60.6).
+    constexpr uint32_t kWide = SRC == SRC_NORM ? 2048 : OUT != OUT_NV ? 768 : SRC == SRC_PLAIN ? 256 : 512;
     if (a.rows < 296 && chunks <= 1024) fp4_row_kernel<SRC, T, OUT, 1><<<grid, threads(1), 0, st>>>(a);
-    else if (chunks <= 2048) fp4_row_kernel<SRC, T, OUT, 2><<<grid, threads(2), 0, st>>>(a);
+    else if (chunks <= kWide) fp4_row_kernel<SRC, T, OUT, 2><<<grid, threads(2), 0, st>>>(a);
     else fp4_row_kernel<SRC, T, OUT, 4><<<grid, threads(4), 0, st>>>(a);
     return launch_status();
 }

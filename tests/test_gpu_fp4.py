@@ -335,3 +335,60 @@ def test_linear_whole_rounds_and_a_rest(fmt, dtype, m, n, k):
     check_product(got[rows], av[rows], wv, None, dtype)
     cols = sorted({0, 255, 256, n // 2, n - 513, n - 257, n - 256, n - 129, n - 1})
     check_product(got[:, cols], av, wv[cols], None, dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,cols", [(20000, 96), (5000, 1056), (1500, 8192), (700, 16416), (400, 28672), (160, 65536)])
+def test_many_rows(fmt, rows, cols):
+    """More rows than CTAs fit, so that a CTA does several: the first, the last and some between against the definition, the SiLU
+    product and the norm (in place too) against their steps."""
+    dtype = torch.bfloat16 if rows % 400 else torch.float16
+    x = make(rows, cols, dtype, rows)
+    pick = sorted({0, 1, rows // 3, rows // 2, 591, 592, 593, rows - 2, rows - 1} & set(range(rows)))
+    codes, tiled, row = ops().fp4_quantize(fmt, x.cuda())
+    c, b, r = F.quantize(fmt, x[pick].double().numpy())
+    assert np.array_equal(F.unpack(codes.cpu().numpy()[pick]), c)
+    assert np.array_equal(F.untile(tiled.cpu().numpy(), rows, cols // F.BLOCK[fmt])[pick], b)
+    assert fmt == "mxfp4" or np.array_equal(row.cpu().numpy()[pick].astype(np.float64), r)
+    xs = x.cuda()
+    gu = torch.cat([xs, xs.flip(0)], 1)
+    h = torch.nn.functional.silu(xs) * xs.flip(0)
+    same(fmt, ops().fp4_silu_mul_quantize(fmt, gu), ops().fp4_quantize(fmt, h), rows, cols)
+    w = (1 + 0.1 * make(1, cols, torch.float32, 3, False)[0]).to(dtype).cuda()
+    for post in (None, w.flip(0)):
+        r, h = _joint(xs, w, 1e-5, xs.flip(0), post, None, 0.5)
+        got = ops().norm_residual_quantize(fmt, xs, w, 1e-5, xs.flip(0), post, None, 0.5)
+        assert torch.equal(got[0], r)
+        same(fmt, got[1:], ops().fp4_quantize(fmt, h), rows, cols)
+    h = _joint(xs, w, 1e-5, None, None, None, 1.0)[1]
+    same(fmt, ops().norm_residual_quantize(fmt, xs, w, 1e-5)[1:], ops().fp4_quantize(fmt, h), rows, cols)
+
+
+def same(fmt, a, b, rows, cols):
+    assert torch.equal(a[0], b[0])
+    blocks = cols // F.BLOCK[fmt]
+    assert np.array_equal(F.untile(a[1].cpu().numpy(), rows, blocks), F.untile(b[1].cpu().numpy(), rows, blocks))
+    assert a[2] is None if fmt == "mxfp4" else torch.equal(a[2], b[2])
+
+
+@pytest.mark.parametrize("rows,cols", [(3, 256), (900, 8192)])
+@pytest.mark.parametrize("into", ["residual", "x"])
+def test_norm_in_place(rows, cols, into):
+    """residual_out may be the residual or x itself (C entry point)."""
+    import ctypes
+    import duqlinear4bitcuda_b200.lib as L
+    x, residual = make(rows, cols, torch.bfloat16, 1).cuda(), make(rows, cols, torch.bfloat16, 2).cuda()
+    w = (1 + 0.1 * make(1, cols, torch.float32, 3, False)[0]).to(torch.bfloat16).cuda()
+    r, h = _joint(x, w, 1e-6, residual, w, w, 0.25)
+    n = L.NormResidual()
+    n.dtype, n.residual_scale, n.clip_ratio, n.eps = L.DTYPE_BF16, 0.25, 1.0, 1e-6
+    n.x, n.residual, n.post_weight, n.gate, n.weight = x.data_ptr(), residual.data_ptr(), w.data_ptr(), w.data_ptr(), w.data_ptr()
+    target = residual if into == "residual" else x
+    n.residual_out = target.data_ptr()
+    out = torch.empty_like(x)
+    L.call("duq4_norm_residual_quantize", 0, ctypes.byref(n), rows, cols, L.ptr(out), None, None, L.current_stream())
+    torch.cuda.synchronize()
+    assert torch.equal(target, r) and torch.equal(out, h)
+    status = ctypes.c_int32(-1)
+    L.call("duq4_last_device_status", L.current_stream(), ctypes.byref(status))
+    assert status.value == 0
