@@ -153,6 +153,7 @@ __device__ __forceinline__ void leave_copies_behind() {   // a producer that giv
 struct PairArgs {
     GemmArgs g;
     uint32_t tiles_m, tiles_n, bn;   // tiles of 256 tokens x bn channels (128 or 256)
+    uint32_t early;                  // 1: the tokens' quantizer is the launch in front and may still run
 };
 
 template <int FMT>
@@ -273,7 +274,9 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         tm = band * 16 + r % here;
     };
 
-    if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the rest of the columns, where a second launch does them
+    if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
+    // the rest of the columns, where a second launch does them, may start: the tokens are there
+    if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
         if (lane == 0) {
             uint32_t it = 0;
@@ -632,7 +635,7 @@ static int launch(F *kernel, uint32_t gx, uint32_t gy, uint32_t threads, uint32_
 }
 
 template <int FMT, class T>
-static int launch_pair(const GemmArgs &g, cudaStream_t st) {
+static int launch_pair(const GemmArgs &g, cudaStream_t st, uint32_t early) {
     using C = Pair<FMT>;
     static DeviceOnce once;
     const int dev = current_device_slot();
@@ -640,7 +643,7 @@ static int launch_pair(const GemmArgs &g, cudaStream_t st) {
     int rc = once.run(dev, [] { return (int)cudaFuncSetAttribute(fp4_pair_kernel<FMT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
     if (rc) return rc;
     const uint32_t pairs = (uint32_t)sm_count_current_device() / 2;
-    PairArgs p{g, cdiv(g.M, 256), 0, 256};
+    PairArgs p{g, cdiv(g.M, 256), 0, 256, early};
     if ((uint64_t)p.tiles_m * cdiv(g.N, 256) * 2 <= pairs) p.bn = 128;
     p.tiles_n = cdiv(g.N, p.bn);
     CUtensorMap maps[4];
@@ -649,7 +652,7 @@ static int launch_pair(const GemmArgs &g, cudaStream_t st) {
         return rc;
     if ((uint64_t)p.tiles_m * p.tiles_n > 0x7FFFFFFFull) return DUQ4_ERR_SHAPE;
     const uint32_t n = p.tiles_m * p.tiles_n < pairs ? p.tiles_m * p.tiles_n : pairs;
-    return launch(fp4_pair_kernel<FMT, T>, 2 * n, 1, C::kThreads, C::kSmem, 2, false, st, maps, &p);
+    return launch(fp4_pair_kernel<FMT, T>, 2 * n, 1, C::kThreads, C::kSmem, 2, early != 0, st, maps, &p);
 }
 
 // CTAs that share a tile's K: up to eight while there is an SM for each (M 16, 4096 x 4096: 9.0 / 8.3 / 7.5 / 7.6 us with 1 / 2 / 4 /
@@ -704,11 +707,6 @@ static uint64_t swap_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
 }
 template <int FMT, class T>
 static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
-#ifdef FORCE_PAIR
-    return launch_pair<FMT, T>(a, st);
-#elif defined(FORCE_SWAP)
-    return launch_swap<FMT, T>(a, st, overlap);
-#endif
     if (a.M <= 128) return launch_swap<FMT, T>(a, st, overlap);
     const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK), tiles_m = cdiv(a.M, 256), tiles_n = cdiv(a.N, 256);
     const uint64_t all = pair_price(tiles_m * tiles_n, ktiles, sms), blocks_m = cdiv(a.M, 128);
@@ -728,11 +726,11 @@ static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
             if (a.w_rows) left.w_rows += n0;
             if (a.bias) left.bias = reinterpret_cast<const uint16_t *>(a.bias) + n0;
             left.out = reinterpret_cast<uint16_t *>(a.out) + n0;
-            const int rc = launch_pair<FMT, T>(main, st);
+            const int rc = launch_pair<FMT, T>(main, st, overlap);
             return rc ? rc : launch_swap<FMT, T>(left, st, 2);
         }
     }
-    return launch_pair<FMT, T>(a, st);
+    return launch_pair<FMT, T>(a, st, overlap);
 }
 
 static int check_gemm(int format, int dtype, uint32_t N, uint32_t K, uint64_t ldo) {
