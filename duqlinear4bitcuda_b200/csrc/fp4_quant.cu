@@ -28,6 +28,7 @@ struct RowArgs {
     uint8_t *codes;               // OUT_ROW: the 16-bit row itself
     uint8_t *block_scales;        // OUT_SYM / OUT_ASYM: fp16 scales [rows]
     void *row_scales;             // OUT_NV: float [rows]; OUT_ASYM: fp16 zero-points [rows]
+    uint32_t lanes;               // threads of a row (narrow rows)
     uint32_t wide;                // every 16-bit tensor and row starts on a 32-byte boundary
 };
 
@@ -111,9 +112,15 @@ __device__ __forceinline__ uint32_t silu_mul_two(uint32_t g, uint32_t u) {
     return Two<T>::down(s.x, s.y) ^ 0x80008000u;
 }
 
-// Sums and maxima over the block; every thread gets the result. `sm` must not be in use by an earlier reduction's readers.
-__device__ __forceinline__ double block_sum(double v, double *sm) {
-    const uint32_t lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+// Sums and maxima over the threads of a row (the block, or `nt` lanes of a warp); every thread gets the result. `sm` must not
+// be in use by an earlier reduction's readers.
+template <bool LANES>
+__device__ __forceinline__ double row_sum(double v, uint32_t nt, double *sm) {
+    if (LANES) {
+        for (uint32_t o = nt >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    }
+    const uint32_t lane = threadIdx.x & 31, warps = nt >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (warps == 1) return v;
@@ -123,8 +130,13 @@ __device__ __forceinline__ double block_sum(double v, double *sm) {
     for (uint32_t o = warps > 16 ? 16 : warps > 8 ? 8 : warps > 4 ? 4 : 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return __shfl_sync(0xffffffffu, v, 0);
 }
-__device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *sm) {
-    const uint32_t lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+template <bool LANES>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t nt, uint32_t *sm) {
+    if (LANES) {
+        for (uint32_t o = nt >> 1; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    }
+    const uint32_t lane = threadIdx.x & 31, warps = nt >> 5;
     v = __reduce_max_sync(0xffffffffu, v);
     if (warps == 1) return v;
     if (lane == 0) sm[threadIdx.x >> 5] = v;
@@ -147,9 +159,9 @@ __device__ __forceinline__ uint32_t chunk_top(const Chunk &c) {   // largest mag
 // S' - S, is exact and so is the rest, x^2 - (S' - S), which is summed beside it (Dekker's fast two-sum): four
 // operations a value, and an error of the square of a rounding. The threads' sums meet in 64 bits. Rows whose squares
 // leave the range of 32 bits (bfloat16 beyond 1e18 or below 1e-15, infinities, NaNs) are summed in 64 bits instead.
-// `again`: where the thread finds its row once more for that.
-template <class T, int CH>
-__device__ __forceinline__ float row_rstd(const Chunk (&d)[CH], const RowArgs &a, const uint16_t *again, double *sm) {
+// `again`: where the thread, tid of the row's nt, finds its row once more for that.
+template <class T, int CH, bool LANES>
+__device__ __forceinline__ float row_rstd(const Chunk (&d)[CH], const RowArgs &a, const uint16_t *again, uint32_t tid, uint32_t nt, double *sm) {
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < CH; ++i) top = max(top, chunk_top<T>(d[i]));
@@ -172,37 +184,44 @@ __device__ __forceinline__ float row_rstd(const Chunk (&d)[CH], const RowArgs &a
     if (odd) {
         sum = 0;
 #pragma unroll 1
-        for (uint32_t c = threadIdx.x; c < a.cols >> 4; c += blockDim.x)
+        for (uint32_t c = tid; c < a.cols >> 4; c += nt)
 #pragma unroll 1
             for (int k = 0; k < 8; ++k) {
                 const float2 x = Two<T>::up(reinterpret_cast<const volatile uint32_t *>(again + c * 16)[k]);
                 sum += (double)x.x * x.x + (double)x.y * x.y;
             }
     }
-    const double v = block_sum(sum, sm) * a.inv_cols + a.eps;
+    const double v = row_sum<LANES>(sum, nt, sm) * a.inv_cols + a.eps;
     if (!(v > 1e-30 && v < 1e30)) return (float)(1.0 / sqrt(v));
     // one Newton step in 64 bits from the 32-bit root: relative error about 1e-14
     const double r = (double)rsqrtf((float)v);
     return (float)(r + r * (0.5 - 0.5 * v * r * r));
 }
 
-// One CTA per row, CH chunks per thread.
-template <int SRC, class T, int OUT, int CH>
-__global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
+// CH chunks per thread. A row is a CTA's, or -- LANES, narrow rows -- that of `lanes` (8, 16 or 32) lanes of a warp, which
+// need no barrier to meet.
+template <int SRC, class T, int OUT, int CH, bool LANES>
+__global__ void __launch_bounds__(LANES ? 256 : 1024, LANES ? 4 : 1) fp4_row_kernel(const RowArgs a) {
     __shared__ double sm_d[2][32];
     __shared__ uint32_t sm_u[32];
     __shared__ float sm_f[32][4];
-    const uint32_t chunks = a.cols >> 4, NT = blockDim.x;
+    const uint32_t chunks_all = a.cols >> 4, NT = LANES ? a.lanes : blockDim.x, tid = LANES ? threadIdx.x & (NT - 1) : threadIdx.x;
     const int lane = threadIdx.x & 31;
     const bool wide = a.wide != 0;
     // a product launched behind the quantizer may start and fetch its weights (nothing happens without such a launch)
     if (SRC == SRC_PLAIN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    // LANES: a warp's rows are neighbours; it goes on together until none of them exists
+    const uint32_t per_warp = LANES ? 32 / NT : 1, mine = LANES ? lane / NT : 0;
+    const uint32_t first = LANES ? (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * per_warp : blockIdx.x;
+    const uint32_t step = LANES ? gridDim.x * (blockDim.x >> 5) * per_warp : gridDim.x;
+    for (uint64_t at = first; at < a.rows; at += step) {
+        const bool there = at + mine < a.rows;
+        const uint32_t row = there ? (uint32_t)(at + mine) : a.rows - 1, chunks = there ? chunks_all : 0;
         Chunk d[CH];
         const uint16_t *xr = a.x + (size_t)row * a.ldx;
 #pragma unroll
         for (int i = 0; i < CH; ++i) {
-            const uint32_t c = threadIdx.x + i * NT;
+            const uint32_t c = tid + i * NT;
             if (c < chunks) {
                 d[i] = load_chunk(xr + c * 16, wide);
                 if (SRC == SRC_SILU) {
@@ -219,10 +238,10 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
             const size_t base = (size_t)row * a.cols;
             if (a.residual) {
                 float rstd = 1.f;
-                if (a.post_weight) rstd = row_rstd<T, CH>(d, a, xr, sm_d[0]);
+                if (a.post_weight) rstd = row_rstd<T, CH, LANES>(d, a, xr, tid, NT, sm_d[0]);
 #pragma unroll
                 for (int i = 0; i < CH; ++i) {
-                    const uint32_t c = threadIdx.x + i * NT;
+                    const uint32_t c = tid + i * NT;
                     if (c >= chunks) continue;
                     const Chunk r = load_chunk(a.residual + base + c * 16, wide);
                     Pair2 y[8];
@@ -247,10 +266,10 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
                     store_chunk(a.residual_out + base + c * 16, d[i], wide);
                 }
             }
-            const float rstd = row_rstd<T, CH>(d, a, a.residual ? a.residual_out + base : xr, sm_d[1]);
+            const float rstd = row_rstd<T, CH, LANES>(d, a, a.residual ? a.residual_out + base : xr, tid, NT, sm_d[1]);
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                const uint32_t c = threadIdx.x + i * NT;
+                const uint32_t c = tid + i * NT;
                 if (c >= chunks) continue;
                 const Chunk w = load_chunk(a.weight + c * 16, wide);
 #pragma unroll
@@ -263,10 +282,11 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
         if (OUT == OUT_ROW) {
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                const uint32_t c = threadIdx.x + i * NT;
+                const uint32_t c = tid + i * NT;
                 if (c < chunks) store_chunk(reinterpret_cast<uint16_t *>(a.codes) + (size_t)row * a.cols + c * 16, d[i], wide);
             }
-        } else if (OUT == OUT_SYM || OUT == OUT_ASYM) {
+        } else if constexpr (OUT == OUT_SYM || OUT == OUT_ASYM) {
+            static_assert(!LANES, "the integer formats' statistics meet in the block");
             // the framework's integer formats: statistics, scale and codes of quant_fused_vec_kernel on the row h
             constexpr int MODE = OUT == OUT_SYM ? QSYM : QASYM;
             Stats st;
@@ -274,7 +294,7 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
             uint32_t am = 0;
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                if (threadIdx.x + i * NT >= chunks) continue;
+                if (tid + i * NT >= chunks) continue;
                 am = max(am, chunk_top<T>(d[i]));
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -291,7 +311,7 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
             const FastQ fq = make_fastq<MODE>(r, special);
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                const uint32_t c = threadIdx.x + i * NT;
+                const uint32_t c = tid + i * NT;
                 if (c >= chunks) continue;
                 const uint4 lo = make_uint4(d[i].w[0], d[i].w[1], d[i].w[2], d[i].w[3]);
                 const uint4 hi = make_uint4(d[i].w[4], d[i].w[5], d[i].w[6], d[i].w[7]);
@@ -312,17 +332,17 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
                     const uint32_t t = chunk_top<T>(d[i]);
                     if (t < Two<T>::kInf) top = max(top, t);
                 }
-                top = block_max(top, sm_u);
+                top = row_max<LANES>(top, NT, sm_u);
                 // 8 bits, so that 6 * row_scale and block scale * row_scale are exact
                 row_scale = __bfloat162float(__float2bfloat16_rn(__fdiv_rn(Two<T>::up1(top), 2688.f)));
                 row_scale = fmaxf(row_scale, 7.703719777548943e-34f);   // 2^-110
-                if (threadIdx.x == 0) reinterpret_cast<float *>(a.row_scales)[row] = row_scale;
+                if (tid == 0 && there) reinterpret_cast<float *>(a.row_scales)[row] = row_scale;
                 six = 6.f * row_scale;
                 inv6 = __fdiv_rn(1.f, six);
             }
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
-                const uint32_t c = threadIdx.x + i * NT;
+                const uint32_t c = tid + i * NT;
                 uint32_t top = chunk_top<T>(d[i]);
                 if (FMT == kMX) top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 const bool special = top >= Two<T>::kInf;
@@ -372,7 +392,7 @@ __global__ void __launch_bounds__(1024, 1) fp4_row_kernel(const RowArgs a) {
                     *reinterpret_cast<uint32_t *>(scales + c / (4 * kStep) * 512) = scale;
             }
         }
-        __syncthreads();   // the reductions' buffers are free for the next row
+        if (!LANES) __syncthreads();   // the reductions' buffers are free for the next row
     }
 }
 
@@ -431,9 +451,20 @@ static int launch_rows(RowArgs a, cudaStream_t st) {
     // 35.8 / 31.5, 4096 x 8192 40.1 / 41.8; mxfp4: 2048 x 11008 10.8 / 10.7, silu 26.3 / 28.4, 2048 x 16384 15.9 / 13.9, silu
     // 38.3 / 36.9; norm joint, 2048 x 16384: 55.3 / 60.6).
     constexpr uint32_t kWide = SRC == SRC_NORM ? 2048 : OUT != OUT_NV ? 768 : SRC == SRC_PLAIN ? 256 : 512;
-    if (a.rows < 296 && chunks <= 1024) fp4_row_kernel<SRC, T, OUT, 1><<<grid, threads(1), 0, st>>>(a);
-    else if (chunks <= kWide) fp4_row_kernel<SRC, T, OUT, 2><<<grid, threads(2), 0, st>>>(a);
-    else fp4_row_kernel<SRC, T, OUT, 4><<<grid, threads(4), 0, st>>>(a);
+    // Narrow rows, and enough of them for every SM: lanes of a warp (us with CTAs / lanes, mxfp4: 65536 x 128 16.0 / 5.9, norm
+    // joint 69.9 / 16.4; 32768 x 512 12.1 / 10.7, 38.6 / 32.0; wider rows on a warp, two or four chunks a lane, 16384 x 1024:
+    // 11.2 / 8.4, 25.5 / 28.4; 8192 x 2048: 9.7 / 8.7, 26.9 / 35.1).
+    if constexpr (OUT != OUT_SYM && OUT != OUT_ASYM) {
+        if (chunks <= 32 && a.rows >= 296) {
+            a.lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
+            const uint64_t blocks = ((uint64_t)a.rows * a.lanes + 255) / 256;
+            fp4_row_kernel<SRC, T, OUT, 1, true><<<blocks < 148u * 64u ? (uint32_t)blocks : 148u * 64u, 256, 0, st>>>(a);
+            return launch_status();
+        }
+    }
+    if (a.rows < 296 && chunks <= 1024) fp4_row_kernel<SRC, T, OUT, 1, false><<<grid, threads(1), 0, st>>>(a);
+    else if (chunks <= kWide) fp4_row_kernel<SRC, T, OUT, 2, false><<<grid, threads(2), 0, st>>>(a);
+    else fp4_row_kernel<SRC, T, OUT, 4, false><<<grid, threads(4), 0, st>>>(a);
     return launch_status();
 }
 

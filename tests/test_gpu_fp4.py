@@ -392,3 +392,45 @@ def test_norm_in_place(rows, cols, into):
     status = ctypes.c_int32(-1)
     L.call("duq4_last_device_status", L.current_stream(), ctypes.byref(status))
     assert status.value == 0
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows,cols", [(296, 32), (301, 96), (297, 128), (4001, 160), (1003, 256), (999, 288), (12345, 512)])
+def test_narrow_rows(fmt, rows, cols):
+    """Several rows a warp, ragged ends: all rows against the definition, the SiLU product and the norm against their steps, and
+    nothing written behind the last row."""
+    dtype = torch.float16 if rows % 2 else torch.bfloat16
+    x = make(rows, cols, dtype, rows)
+    x[rows // 2] = 0
+    x[rows - 1, 3] = float("inf")
+    got = ops().fp4_quantize(fmt, x.cuda())
+    check_quantized(fmt, got, x.double().numpy())
+    xs = x.cuda()
+    xs[rows - 1, 3] = 1
+    gu = torch.cat([xs, xs.flip(0)], 1)
+    same(fmt, ops().fp4_silu_mul_quantize(fmt, gu), ops().fp4_quantize(fmt, torch.nn.functional.silu(xs) * xs.flip(0)), rows, cols)
+    w = (1 + 0.1 * make(1, cols, torch.float32, 3, False)[0]).to(dtype).cuda()
+    r, h = _joint(xs, w, 1e-5, xs.flip(0), w.flip(0), xs, 0.5)
+    got = ops().norm_residual_quantize(fmt, xs, w, 1e-5, xs.flip(0), w.flip(0), xs, 0.5)
+    assert torch.equal(got[0], r)
+    same(fmt, got[1:], ops().fp4_quantize(fmt, h), rows, cols)
+
+
+@pytest.mark.parametrize("fmt,rows,cols", [("mxfp4", 300, 96), ("nvfp4", 333, 160), ("nvfp4", 130, 4128), ("mxfp4", 5, 64)])
+def test_quantizer_leaves_what_is_not_its_own(fmt, rows, cols):
+    """Rows read with a stride; codes, scales and row scales behind the last row stay as they were, scale bytes of rows that do
+    not exist too."""
+    import duqlinear4bitcuda_b200.lib as L
+    wide = make(rows, cols + 8, torch.bfloat16, 4).cuda()
+    f = L.FP4_MX if fmt == "mxfp4" else L.FP4_NV
+    size = L.cdll.duq4_fp4_scale_bytes(f, rows, cols)
+    codes = torch.full((rows * cols // 2 + 512,), 0xA5, dtype=torch.uint8, device="cuda")
+    scales = torch.full((size + 512,), 0xA5, dtype=torch.uint8, device="cuda")
+    row = torch.full((rows + 8,), -7.0, device="cuda")
+    L.call("duq4_fp4_quantize", f, L.DTYPE_BF16, L.ptr(wide), rows, cols, cols + 8, L.ptr(codes), L.ptr(scales), L.ptr(row), L.current_stream())
+    want = ops().fp4_quantize(fmt, wide[:, :cols].contiguous())
+    assert torch.equal(codes[:rows * cols // 2].view(rows, -1), want[0]) and (codes[rows * cols // 2:] == 0xA5).all()
+    assert (scales[size:] == 0xA5).all() and (row[rows:] == -7).all()
+    padded = -(-(cols // F.BLOCK[fmt]) // 4) * 4
+    t = F.untile(scales[:size].cpu().numpy(), -(-rows // 128) * 128, padded)
+    assert (t[rows:] == 0xA5).all() and np.array_equal(t[:rows], F.untile(want[1].cpu().numpy(), rows, padded))
