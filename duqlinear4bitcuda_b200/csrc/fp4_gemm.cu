@@ -20,6 +20,9 @@ namespace duq4 {
 
 __device__ int g_fp4_status = 0;
 
+int fp4_quantize_rows(int format, int dtype, const void *x, uint32_t rows, uint32_t cols, uint64_t ldx, uint8_t *codes, uint8_t *block_scales,
+                      float *row_scales, cudaStream_t st);
+
 namespace fp4 {
 
 using namespace ptx;
@@ -504,10 +507,10 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
         }
     } else {
-        if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");
         wait(acc_full, 0, abortp, 13);
         tc_fence_after();
     }
+    if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens' factors
     if (warp >= 2 && !abort_flag) {
         const uint32_t quad = warp & 3, acc = tmem + ((quad * 32) << 16);
         for (uint32_t c = 0; c < p.nt; c += 16) {
@@ -687,7 +690,10 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, uint32_t early) {
     uint32_t smem = p.stages * per_stage;
     if (smem < p.nt * 512u) smem = p.nt * 512u;
     smem += 1024;
-    if (tiles_m > 65535) return DUQ4_ERR_SHAPE;
+    // A CTA takes at least as large a part of the SM's shared memory as of its TMEM (64 columns count for a ninth of 228 KiB), so
+    // that CTAs whose columns do not fit together are never on one SM together: one that waited there for columns would keep
+    // its cluster waiting, and the cluster what others wait for.
+    if (smem < p.tmem_cols * 408u) smem = p.tmem_cols * 408u;
     CUtensorMap maps[4];
     if ((rc = map_codes(&maps[0], g.a, g.M, g.K, p.nt)) || (rc = map_codes(&maps[1], g.w, g.N, g.K, 128)) ||
         (rc = map_scales(&maps[2], g.a_scales, FMT, g.M, g.K, 1)) || (rc = map_scales(&maps[3], g.w_scales, FMT, g.N, g.K, 1)))
@@ -710,11 +716,12 @@ static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
     if (a.M <= 128) return launch_swap<FMT, T>(a, st, overlap);
     const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK), tiles_m = cdiv(a.M, 256), tiles_n = cdiv(a.N, 256);
     const uint64_t all = pair_price(tiles_m * tiles_n, ktiles, sms), blocks_m = cdiv(a.M, 128);
-    if (swap_price(blocks_m * cdiv(a.N, 128), ktiles, sms) < all) return launch_swap<FMT, T>(a, st, overlap);
+    const bool swap_fits = blocks_m <= 65535;   // the grid's second dimension
+    if (swap_fits && swap_price(blocks_m * cdiv(a.N, 128), ktiles, sms) < all) return launch_swap<FMT, T>(a, st, overlap);
     // A last round that few tiles are left for: whole rounds by the pair kernel, the columns that are left by the other one,
     // launched behind it (512 x 28672 x 8192, 3 rounds and 2 tiles of 256 x 256: 57.9 -> 53.3 us).
     const uint64_t rest = tiles_m * tiles_n % (sms / 2), strip = rest ? (rest + tiles_m - 1) / tiles_m : 0;
-    if (strip && strip < tiles_n) {
+    if (swap_fits && strip && strip < tiles_n) {
         const uint32_t n0 = (uint32_t)(tiles_n - strip) * 256;
         const uint64_t both = pair_price(tiles_m * (tiles_n - strip), ktiles, sms) + swap_price(blocks_m * cdiv(a.N - n0, 128), ktiles, sms);
         if (both < all) {
@@ -733,10 +740,10 @@ static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
     return launch_pair<FMT, T>(a, st, overlap);
 }
 
-static int check_gemm(int format, int dtype, uint32_t N, uint32_t K, uint64_t ldo) {
+static int check_gemm(int format, int dtype, uint32_t M, uint32_t N, uint32_t K, uint64_t ldo) {
     if (format != kMX && format != kNV) return DUQ4_ERR_MODE;
     if (dtype != DUQ4_DTYPE_F16 && dtype != DUQ4_DTYPE_BF16) return DUQ4_ERR_MODE;
-    if (K == 0 || K % 32 != 0 || ldo < N) return DUQ4_ERR_SHAPE;
+    if (K == 0 || K % 32 != 0 || ldo < N || (M | N | K) > 0x7FFFFFFFu) return DUQ4_ERR_SHAPE;
     return DUQ4_OK;
 }
 static bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -774,7 +781,7 @@ int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales,
                     void *out, uint64_t ldo, void *stream) {
     DUQ4_TRACE();
     if (ldo == 0) ldo = N;
-    int rc = check_gemm(format, dtype, N, K, ldo);
+    int rc = check_gemm(format, dtype, M, N, K, ldo);
     if (rc) return rc;
     if (M == 0 || N == 0) return DUQ4_OK;
     if (!A || !A_block_scales || !W || !W_block_scales || !out) return DUQ4_ERR_NULL;
@@ -794,7 +801,7 @@ int duq4_linear_fp4_from_16bit(int format, int dtype, const void *x, const uint8
                                void *workspace, size_t workspace_bytes, void *stream) {
     DUQ4_TRACE();
     if (ldo == 0) ldo = N;
-    int rc = check_gemm(format, dtype, N, K, ldo);
+    int rc = check_gemm(format, dtype, M, N, K, ldo);
     if (rc) return rc;
     if (M == 0 || N == 0) return DUQ4_OK;
     if (!x || !W || !W_block_scales || !out) return DUQ4_ERR_NULL;
@@ -802,7 +809,7 @@ int duq4_linear_fp4_from_16bit(int format, int dtype, const void *x, const uint8
     if (!aligned(W, 16) || !aligned(W_block_scales, 16) || !aligned(W_row_scales, 4) || !aligned(bias, 2) || !aligned(out, 2)) return DUQ4_ERR_ALIGN;
     uint8_t *codes = (uint8_t *)workspace, *scales = codes + up256((size_t)M * (K / 2));
     float *rows = format == kNV ? (float *)(scales + up256(duq4_fp4_scale_bytes(format, M, K))) : nullptr;
-    rc = duq4_fp4_quantize(format, dtype, x, M, K, K, codes, scales, rows, stream);
+    rc = fp4_quantize_rows(format, dtype, x, M, K, K, codes, scales, rows, (cudaStream_t)stream);
     if (rc) return rc;
     const GemmArgs a{M, N, K, codes, scales, W, W_block_scales, rows, W_row_scales, bias, out, ldo};
     // The product may start while the quantizer runs: the quantizer is an ordinary launch, so everything that was queued

@@ -482,6 +482,24 @@ static int quantize_rows(int format, int dtype, const RowArgs &a, cudaStream_t s
 }
 
 }  // namespace fp4
+
+// duq4_fp4_quantize without its trace range: also the first half of duq4_linear_fp4_from_16bit.
+int fp4_quantize_rows(int format, int dtype, const void *x, uint32_t rows, uint32_t cols, uint64_t ldx, uint8_t *codes,
+                      uint8_t *block_scales, float *row_scales, cudaStream_t st) {
+    using namespace fp4;
+    int rc = check_fp4(format, dtype, cols);
+    if (rc) return rc;
+    if (rows == 0) return DUQ4_OK;
+    if (!x || !codes || !block_scales || (format == kNV && !row_scales)) return DUQ4_ERR_NULL;
+    if (ldx < cols || ldx % 8 != 0) return DUQ4_ERR_SHAPE;
+    if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(block_scales, 16) || !aligned(row_scales, 4)) return DUQ4_ERR_ALIGN;
+    RowArgs a{};
+    a.rows = rows; a.cols = cols; a.ldx = ldx;
+    a.x = (const uint16_t *)x;
+    a.codes = codes; a.block_scales = block_scales; a.row_scales = row_scales;
+    return quantize_rows<SRC_PLAIN>(format, dtype, a, st);
+}
+
 }  // namespace duq4
 
 using namespace duq4;
@@ -497,17 +515,7 @@ size_t duq4_fp4_scale_bytes(int format, uint32_t rows, uint32_t cols) {
 int duq4_fp4_quantize(int format, int dtype, const void *x, uint32_t rows, uint32_t cols, uint64_t ldx, uint8_t *codes,
                       uint8_t *block_scales, float *row_scales, void *stream) {
     DUQ4_TRACE();
-    int rc = check_fp4(format, dtype, cols);
-    if (rc) return rc;
-    if (rows == 0) return DUQ4_OK;
-    if (!x || !codes || !block_scales || (format == kNV && !row_scales)) return DUQ4_ERR_NULL;
-    if (ldx < cols || ldx % 8 != 0) return DUQ4_ERR_SHAPE;
-    if (!aligned(x, 16) || !aligned(codes, 16) || !aligned(block_scales, 16) || !aligned(row_scales, 4)) return DUQ4_ERR_ALIGN;
-    RowArgs a{};
-    a.rows = rows; a.cols = cols; a.ldx = ldx;
-    a.x = (const uint16_t *)x;
-    a.codes = codes; a.block_scales = block_scales; a.row_scales = row_scales;
-    return quantize_rows<SRC_PLAIN>(format, dtype, a, (cudaStream_t)stream);
+    return fp4_quantize_rows(format, dtype, x, rows, cols, ldx, codes, block_scales, row_scales, (cudaStream_t)stream);
 }
 
 int duq4_fp4_silu_mul_quantize(int format, int dtype, const void *gate_up, uint32_t rows, uint32_t inter, uint64_t ld, uint32_t up_offset,

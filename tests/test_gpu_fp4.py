@@ -434,3 +434,145 @@ def test_quantizer_leaves_what_is_not_its_own(fmt, rows, cols):
     padded = -(-(cols // F.BLOCK[fmt]) // 4) * 4
     t = F.untile(scales[:size].cpu().numpy(), -(-rows // 128) * 128, padded)
     assert (t[rows:] == 0xA5).all() and np.array_equal(t[:rows], F.untile(want[1].cpu().numpy(), rows, padded))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 32), (1, 2, 64), (5, 7, 96), (129, 1, 288), (300, 3, 1056), (257, 255, 32), (16, 4096, 65536)])
+def test_linear_smallest_and_longest(fmt, m, n, k):
+    ap, at, ar, av = F.random_operand(fmt, m, k, 1)
+    wp, wt, wr, wv = F.random_operand(fmt, n, k, 2)
+    got = ops().linear_fp4(fmt, F.cuda(ap), F.cuda(at), F.cuda(ar), F.cuda(wp), F.cuda(wt), F.cuda(wr), None, torch.bfloat16)
+    check_product(got, av, wv, None, torch.bfloat16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("m", [3, 300])
+def test_linear_writes_its_rows_and_columns_only(fmt, m):
+    """A result with a row stride inside a larger buffer, rows aligned and not; what lies around it stays."""
+    import duqlinear4bitcuda_b200.lib as L
+    n, k = 520, 288
+    ap, at, ar, _ = F.random_operand(fmt, m, k, 1)
+    wp, wt, wr, _ = F.random_operand(fmt, n, k, 2)
+    a, w = [F.cuda(t) for t in (ap, at, ar)], [F.cuda(t) for t in (wp, wt, wr)]
+    want = ops().linear_fp4(fmt, *a, *w, None, torch.bfloat16)
+    f = L.FP4_MX if fmt == "mxfp4" else L.FP4_NV
+    for ldo, first in ((536, 16), (544, 8), (523, 1)):
+        buf = torch.full((m + 2, ldo), 7.0, dtype=torch.bfloat16, device="cuda")
+        L.call("duq4_linear_fp4", f, *map(L.ptr, a), *map(L.ptr, w), m, n, k, None, L.DTYPE_BF16, buf.data_ptr() + 2 * (ldo + first), ldo, L.current_stream())
+        flat = buf.view(-1)
+        got = torch.as_strided(flat, (m, n), (ldo, 1), ldo + first)
+        assert torch.equal(got, want)
+        got.fill_(7.0)
+        assert (buf == 7).all()
+
+
+def test_two_streams_and_threads_at_once():
+    """Products of both kernels and quantizers queued on several streams by several host threads: every result as alone."""
+    import threading
+    jobs = []
+    for i, (fmt, m, n, k) in enumerate([("nvfp4", 4, 4096, 2048), ("mxfp4", 100, 1000, 4096), ("nvfp4", 700, 2000, 1024), ("mxfp4", 128, 512, 8192)]):
+        x = make(m, k, torch.bfloat16, i).cuda()
+        wp, wt, wr, _ = F.random_operand(fmt, n, k, i)
+        args = (fmt, x, F.cuda(wp), F.cuda(wt), F.cuda(wr))
+        jobs.append((args, ops().linear_fp4_from_16bit(*args)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(args, want):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            outs = [ops().linear_fp4_from_16bit(*args) for _ in range(50)]
+        s.synchronize()
+        if not all(torch.equal(o, want) for o in outs):
+            bad.append(args[0])
+    threads = [threading.Thread(target=work, args=j) for j in jobs for _ in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not bad
+    import ctypes
+    import duqlinear4bitcuda_b200.lib as L
+    status = ctypes.c_int32(-1)
+    L.call("duq4_last_device_status", L.current_stream(), ctypes.byref(status))
+    assert status.value == 0
+
+
+def test_captured_products_replay_side_by_side():
+    """Two graphs of from_16bit, one with columns left over behind whole rounds, replayed at once on two streams."""
+    made = []
+    for fmt, m, n, k in (("nvfp4", 300, 9600, 1056), ("mxfp4", 20, 3000, 2048)):
+        x = make(m, k, torch.float16, m).cuda()
+        wp, wt, wr, _ = F.random_operand(fmt, n, k, 3)
+        args = (fmt, x, F.cuda(wp), F.cuda(wt), F.cuda(wr) * 1e-4)
+        want = ops().linear_fp4_from_16bit(*args)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = ops().linear_fp4_from_16bit(*args)
+            out2 = ops().linear_fp4_from_16bit(*args)
+        made.append((g, out, out2, want, torch.cuda.Stream(), args))
+    for _ in range(5):
+        for g, out, out2, want, s, _ in made:
+            with torch.cuda.stream(s):
+                out.zero_()
+                g.replay()
+    torch.cuda.synchronize()
+    for g, out, out2, want, s, _ in made:
+        assert torch.equal(out, want) and torch.equal(out2, want)
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 elements: the last rows of a quantizer, of a product's activations and of its result."""
+    rows, cols = 66000, 65536
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x.view(torch.int16).random_(0x3F00, 0x4080)
+    for fmt in FORMATS:
+        codes, tiled, row = ops().fp4_quantize(fmt, x)
+        some = ops().fp4_quantize(fmt, x[-128 - rows % 128:].contiguous())
+        assert torch.equal(codes[-128 - rows % 128:], some[0])
+        tail = tiled[-some[1].numel():]
+        blocks = cols // F.BLOCK[fmt]
+        assert np.array_equal(F.untile(tail.cpu().numpy(), 128 + rows % 128, blocks), F.untile(some[1].cpu().numpy(), 128 + rows % 128, blocks))
+        assert row is None or torch.equal(row[-200:], some[2][-200:])
+        back = ops().fp4_dequantize(fmt, codes, tiled, row, torch.bfloat16)
+        assert torch.equal(back[-100:], ops().fp4_dequantize(fmt, *some, torch.bfloat16)[-100:])
+        del back
+        wp, wt, wr, _ = F.random_operand(fmt, 40, cols, 3)
+        w = (F.cuda(wp), F.cuda(wt), F.cuda(wr))
+        y = ops().linear_fp4(fmt, codes, tiled, row, *w, None, torch.bfloat16)
+        few = ops().linear_fp4(fmt, *some, *w, None, torch.bfloat16)
+        assert torch.allclose(y[-200:].float(), few[-200:].float(), rtol=2 ** -6, atol=1e-2 * few.float().abs().max().item())
+        del codes, tiled, row, y
+    del x
+    m, n, k = 70000, 65536, 64
+    ap, at, ar, av = F.random_operand("nvfp4", m, k, 1)
+    wp, wt, wr, wv = F.random_operand("nvfp4", n, k, 2)
+    y = ops().linear_fp4("nvfp4", F.cuda(ap), F.cuda(at), F.cuda(ar), F.cuda(wp), F.cuda(wt), F.cuda(wr), None, torch.bfloat16)
+    for r in (0, 65535, 65536, m - 1):
+        check_product(y[r:r + 1], av[r:r + 1], wv, None, torch.bfloat16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_refusals_on_the_gpu(fmt):
+    """Wrong sizes, layouts and alignments of tensors that are on the GPU raise and launch nothing."""
+    o = ops()
+    x = make(8, 128, torch.float16).cuda()
+    q = o.fp4_quantize(fmt, x)
+    w = torch.ones(128, dtype=torch.float16, device="cuda")
+    for call, match in [
+        (lambda: o.fp4_quantize(fmt, x[:, :100].contiguous()), "multiple of 32"),
+        (lambda: o.fp4_quantize(fmt, x.t()), "contiguous"),
+        (lambda: o.fp4_quantize(fmt, torch.empty(4, 65568, dtype=torch.float16, device="cuda")), "shape"),
+        (lambda: o.fp4_quantize(fmt, x.view(-1)[4:4 + 256].view(2, 128)), "aligned"),
+        (lambda: o.fp4_dequantize(fmt, q[0], q[1][:-1], q[2], torch.float16), "bytes"),
+        (lambda: o.fp4_dequantize("nvfp4", q[0], q[1] if fmt == "nvfp4" else o.fp4_quantize("nvfp4", x)[1], None, torch.float16), "row_scales"),
+        (lambda: o.linear_fp4(fmt, *q, q[0][:, :32].contiguous(), q[1], q[2]), "bytes|disagree"),
+        (lambda: o.linear_fp4(fmt, *q, *q, torch.ones(7, dtype=torch.float16, device="cuda")), "bias to have 8 entries"),
+        (lambda: o.linear_fp4_from_16bit(fmt, x[:, :64].contiguous(), *q), "disagree on K"),
+        (lambda: o.norm_residual_quantize(fmt, x, w[:64]), "weight to have 128"),
+        (lambda: o.norm_residual_quantize(fmt, x, w, post_weight=w), "go with residual"),
+        (lambda: o.norm_residual_quantize(fmt, x, w, residual=x[:4]), "disagree on their shape"),
+        (lambda: o.norm_residual_quantize(fmt, x, w, residual=x, gate=x[:4]), "gate must be"),
+        (lambda: o.norm_residual_quantize(fmt, x, w, -1.0), "eps"),
+    ]:
+        with pytest.raises(RuntimeError, match=match):
+            call()
