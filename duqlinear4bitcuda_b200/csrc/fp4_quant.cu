@@ -200,8 +200,8 @@ __device__ __forceinline__ float row_rstd(const Chunk (&d)[CH], const RowArgs &a
 
 // CH chunks per thread. A row is a CTA's, or -- LANES, narrow rows -- that of `lanes` (8, 16 or 32) lanes of a warp, which
 // need no barrier to meet.
-template <int SRC, class T, int OUT, int CH, bool LANES>
-__global__ void __launch_bounds__(LANES ? 256 : 1024, LANES ? 4 : 1) fp4_row_kernel(const RowArgs a) {
+template <int SRC, class T, int OUT, int CH, bool LANES, int REGS>
+__global__ void __maxnreg__(REGS) fp4_row_kernel(const RowArgs a) {
     __shared__ double sm_d[2][32];
     __shared__ uint32_t sm_u[32];
     __shared__ float sm_f[32][4];
@@ -458,13 +458,24 @@ static int launch_rows(RowArgs a, cudaStream_t st) {
         if (chunks <= 32 && a.rows >= 296) {
             a.lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
             const uint64_t blocks = ((uint64_t)a.rows * a.lanes + 255) / 256;
-            fp4_row_kernel<SRC, T, OUT, 1, true><<<blocks < 148u * 64u ? (uint32_t)blocks : 148u * 64u, 256, 0, st>>>(a);
+            fp4_row_kernel<SRC, T, OUT, 1, true, 64><<<blocks < 148u * 64u ? (uint32_t)blocks : 148u * 64u, 256, 0, st>>>(a);
             return launch_status();
         }
     }
-    if (a.rows < 296 && chunks <= 1024) fp4_row_kernel<SRC, T, OUT, 1, false><<<grid, threads(1), 0, st>>>(a);
-    else if (chunks <= kWide) fp4_row_kernel<SRC, T, OUT, 2, false><<<grid, threads(2), 0, st>>>(a);
-    else fp4_row_kernel<SRC, T, OUT, 4, false><<<grid, threads(4), 0, st>>>(a);
+    // Registers a thread may have: fewer where that puts more rows on an SM at little spilling (us with 64 / 56 / 48 / 40 at
+    // 32 columns a thread: mxfp4 4096 x 11008 20.8 / 21.0 / 20.8 / 19.0, silu 60.4 / 50.1 / 50.0 / 46.3; nvfp4 silu 4096 x 8192
+    // 41.1 / 40.9 / 38.9 / 39.0; norm joint 4096 x 11008, whose 352 threads fit twice with 64, three times with 48:
+    // 88.1 / 79.6 / 78.0 / 105.8, but 2048 x 16384 56.4 / 60.8 / 60.4 / 82.4).
+    if (a.rows < 296 && chunks <= 1024) {
+        fp4_row_kernel<SRC, T, OUT, 1, false, 64><<<grid, threads(1), 0, st>>>(a);
+    } else if (chunks <= kWide) {
+        const uint32_t nt = threads(2);
+        constexpr int kRegs = SRC == SRC_NORM ? 64 : OUT == OUT_MX ? 40 : SRC == SRC_SILU ? 48 : 64;
+        if (SRC == SRC_NORM && 1024 / nt * nt < 768) fp4_row_kernel<SRC, T, OUT, 2, false, SRC == SRC_NORM ? 48 : kRegs><<<grid, nt, 0, st>>>(a);
+        else fp4_row_kernel<SRC, T, OUT, 2, false, kRegs><<<grid, nt, 0, st>>>(a);
+    } else {
+        fp4_row_kernel<SRC, T, OUT, 4, false, 64><<<grid, threads(4), 0, st>>>(a);
+    }
     return launch_status();
 }
 
