@@ -576,3 +576,22 @@ def test_refusals_on_the_gpu(fmt):
     ]:
         with pytest.raises(RuntimeError, match=match):
             call()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 22016, 4096), (1, 4096, 11008), (16, 4096, 4096), (2, 129, 32), (16, 40, 96), (7, 300, 2080), (3, 1000, 4128),
+                                   (13, 20000, 1056), (1, 100, 65536), (5, 513, 8192)])
+def test_few_tokens_from_16bit(fmt, dtype, m, n, k):
+    """Few tokens on long and short layers equal quantizer and product, bit for bit; bad tokens and zero tokens among them."""
+    x = make(m, k, dtype, m + k).cuda()
+    if m > 4:
+        x[1] = 0
+        x[2, k - 1] = float("inf")
+        x[3, 0] = float("nan")
+    wp, wt, wr, _ = F.random_operand(fmt, n, k, 11)
+    w = (F.cuda(wp), F.cuda(wt), F.cuda(wr))
+    bias = make(1, n, dtype, 9)[0].cuda()
+    want = ops().linear_fp4(fmt, *ops().fp4_quantize(fmt, x), *w, bias, dtype)
+    got = ops().linear_fp4_from_16bit(fmt, x, *w, bias)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
