@@ -454,6 +454,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         mbar_init(acc_full, 1);
         mbar_init(drained, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_proxy_async();   // the copies find the barriers initialised
         for (uint32_t i = 0; i < head; ++i) {   // before the CTA is set up
             weights(k0 + i, i);
             if (p.early != 1) tokens(k0 + i, i);

@@ -595,3 +595,23 @@ def test_few_tokens_from_16bit(fmt, dtype, m, n, k):
     want = ops().linear_fp4(fmt, *ops().fp4_quantize(fmt, x), *w, bias, dtype)
     got = ops().linear_fp4_from_16bit(fmt, x, *w, bias)
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(), want.nan_to_num())
+
+
+@pytest.mark.parametrize("fmt", ["sym", "asym"])
+@pytest.mark.parametrize("rows,cols", [(2, 65536), (400, 32), (700, 512), (1200, 11008)])
+def test_norm_into_the_integer_layers(fmt, rows, cols):
+    """The integer formats at the widest and the narrowest rows, and on into the layer that takes them."""
+    import duqlinear4bitcuda_b200.nn as nn
+    x, residual = make(rows, cols, torch.float16, 1).cuda(), make(rows, cols, torch.float16, 2).cuda()
+    joint = nn.NormResidualQuantizer(cols, fmt, eps=1e-5, post_norm=True, residual_scale=0.5).cuda()
+    q, stream = joint(x, residual)
+    r, h = _joint(x, joint.weight, 1e-5, residual, joint.post_weight, None, 0.5)
+    assert torch.equal(stream, r)
+    want = (nn.SymQuantizer() if fmt == "sym" else nn.AsymQuantizer())(h)
+    assert torch.equal(q.quantized_x, want.quantized_x) and torch.equal(q.scales_x.flatten(), want.scales_x.flatten())
+    if fmt == "asym":
+        assert torch.equal(q.zeros_x.flatten(), want.zeros_x.flatten())
+    elif cols % 64 == 0:
+        lin = nn.Linear4bitSQ(cols, 64).cuda()
+        lin.weight_scales.fill_(0.01)
+        assert torch.equal(lin(q), lin(want))
