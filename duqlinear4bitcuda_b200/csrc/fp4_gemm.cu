@@ -281,16 +281,15 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     // the rest of the columns, where a second launch does them, may start: the tokens are there
     if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            const uint32_t bytes = 2 * (C::kOperand + bn / 2 * 128 + C::kScaleA * (1 + bn / 128));
-            for (uint32_t t = pair; ok && t < tiles; t += npairs) {
-                uint32_t tm, tn;
-                coords(t, tm, tn);
-                for (uint32_t ks = 0; ks < ksteps; ++ks, ++it) {
-                    const uint32_t s = it % C::kStages, ph = (it / C::kStages) & 1;
-                    if (!(ok = wait(empty(s), ph ^ 1, abortp, 1))) break;
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        const uint32_t bytes = 2 * (C::kOperand + bn / 2 * 128 + C::kScaleA * (1 + bn / 128));
+        for (uint32_t t = pair; ok && t < tiles; t += npairs) {
+            uint32_t tm, tn;
+            coords(t, tm, tn);
+            for (uint32_t ks = 0; ks < ksteps; ++ks) {
+                if (!(ok = wait(empty(s), ph ^ 1, abortp, 1))) break;
+                if (elected()) {
                     if (rank == 0) mbar_expect_tx(full(s), bytes);
                     const uint32_t bar = in_cta(full(s), 0), dst = base + s * 2 * C::kOperand, sc = scales0 + s * C::kScaleStage;
                     load_2d<2>(dst, &map_a, bar, ks * 128, tm * 256 + rank * 128);
@@ -298,12 +297,14 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     load_3d<2>(sc, &map_sa, bar, 0, ks * C::kTiles, tm * 2 + rank);
                     load_3d<2>(sc + C::kScaleA, &map_sw, bar, 0, ks * C::kTiles, tn * (bn / 128));
                 }
+                __syncwarp();
+                if (++s == C::kStages) { s = 0; ph ^= 1; }
             }
-            if (!ok) leave_copies_behind();
         }
+        if (!ok) leave_copies_behind();
     } else if (warp == 1) {
         if (rank == 0) {
-            uint32_t it = 0, lt = 0;
+            uint32_t s = 0, ph = 0, lt = 0;
             bool ok = true, issued = false;
             const bool wide = bn == 256;
             const uint32_t idesc = block_idesc<FMT>(256, bn);
@@ -314,8 +315,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (lt > 0 && !(ok = wait(shared_free, (lt - 1) & 1, abortp, 3))) break;
                 tc_fence_after();
                 const uint32_t d = tmem + buf * C::kSecond;
-                for (uint32_t ks = 0; ks < ksteps; ++ks, ++it) {
-                    const uint32_t s = it % C::kStages, ph = (it / C::kStages) & 1;
+                for (uint32_t ks = 0; ks < ksteps; ++ks) {
                     if (!(ok = wait(full(s), ph, abortp, 4))) break;
                     tc_fence_after();
                     const uint64_t da = desc_a + s * (2 * C::kOperand >> 4), ds = desc_s + s * (C::kScaleStage >> 4);
@@ -333,6 +333,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                     }
                     __syncwarp();
                     issued = true;
+                    if (++s == C::kStages) { s = 0; ph ^= 1; }
                 }
             }
             if (!ok && issued) {
@@ -445,19 +446,25 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         load_2d<1>(base + s * stage + 128 * 128, &map_a, full(s), k * 128, t0);
         load_3d<1>(scales0 + s * 2 * C::kScale + C::kScale, &map_sa, full(s), 0, k * C::kTiles, t0 >> 7);
     };
-    if (threadIdx.x == 0) {
-        abort_flag = 0;
-        for (uint32_t s = 0; s < p.stages; ++s) {
-            mbar_init(full(s), 1);
-            mbar_init(empty(s), 1);
+    if (warp == 0) {
+        if (elected()) {
+            abort_flag = 0;
+            for (uint32_t s = 0; s < p.stages; ++s) {
+                mbar_init(full(s), 1);
+                mbar_init(empty(s), 1);
+            }
+            mbar_init(acc_full, 1);
+            mbar_init(drained, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            fence_proxy_async();   // the copies find the barriers initialised
         }
-        mbar_init(acc_full, 1);
-        mbar_init(drained, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        fence_proxy_async();   // the copies find the barriers initialised
+        __syncwarp();
         for (uint32_t i = 0; i < head; ++i) {   // before the CTA is set up
-            weights(k0 + i, i);
-            if (p.early != 1) tokens(k0 + i, i);
+            if (elected()) {
+                weights(k0 + i, i);
+                if (p.early != 1) tokens(k0 + i, i);
+            }
+            __syncwarp();
         }
     }
     if (warp == 1) {
@@ -471,26 +478,31 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     volatile int *abortp = &abort_flag;
 
     if (warp == 0) {
-        if (lane == 0) {
-            bool ok = true;
-            if (p.early == 1) {
-                asm volatile("griddepcontrol.wait;" ::: "memory");
-                for (uint32_t i = 0; i < head; ++i) tokens(k0 + i, i);
+        bool ok = true;
+        if (p.early == 1) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            for (uint32_t i = 0; i < head; ++i) {
+                if (elected()) tokens(k0 + i, i);
+                __syncwarp();
             }
-            for (uint32_t i = head; i < k1 - k0; ++i) {
-                const uint32_t s = i % p.stages, ph = (i / p.stages) & 1;
-                if (!(ok = wait(empty(s), ph ^ 1, abortp, 11))) break;
+        }
+        uint32_t s = 0, ph = 1;
+        for (uint32_t i = head; i < k1 - k0; ++i) {
+            if (!(ok = wait(empty(s), ph ^ 1, abortp, 11))) break;
+            if (elected()) {
                 weights(k0 + i, s);
                 tokens(k0 + i, s);
             }
-            if (!ok) leave_copies_behind();
+            __syncwarp();
+            if (++s == p.stages) { s = 0; ph ^= 1; }
         }
+        if (!ok) leave_copies_behind();
     } else if (warp == 1) {
         bool ok = true, issued = false;
         const uint32_t idesc = block_idesc<FMT>(128, p.nt);
         const uint64_t desc_w = make_desc(base), desc_s = scale_desc(scales0);
+        uint32_t s = 0, ph = 0;
         for (uint32_t i = 0; i < k1 - k0; ++i) {
-            const uint32_t s = i % p.stages, ph = (i / p.stages) & 1;
             if (!(ok = wait(full(s), ph, abortp, 12))) break;
             tc_fence_after();
             const uint64_t dw = desc_w + s * (stage >> 4), ds = desc_s + s * (2 * C::kScale >> 4);
@@ -501,6 +513,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             }
             __syncwarp();
             issued = true;
+            if (++s == p.stages) { s = 0; ph ^= 1; }
         }
         if (!ok && issued) {
             if (elected()) commit<1>(drained);
