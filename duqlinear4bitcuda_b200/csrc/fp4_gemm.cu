@@ -12,6 +12,8 @@
 //                     decode step streams weights and wastes no MMA on absent tokens; K is split over a cluster
 #include <cuda.h>
 
+#include <type_traits>
+
 #include "fp4_common.cuh"
 #include "gemm_tc_shared.cuh"
 #include "trace_range.h"
@@ -436,6 +438,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t tn = blockIdx.x / p.splits, t0 = blockIdx.y * p.nt;
     const uint32_t ktiles = (p.g.K + kBK - 1) / kBK, k0 = rank * ktiles / p.splits, k1 = (rank + 1) * ktiles / p.splits;
 
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the next launch on the stream may set itself up; it waits for this one
     const uint32_t head = min(p.stages, k1 - k0);   // the first round of stages
     auto weights = [&](uint32_t k, uint32_t s) {    // a stage's weights, and the bytes it waits for
         mbar_expect_tx(full(s), stage + 2 * C::kScale);
@@ -459,24 +462,40 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             fence_proxy_async();   // the copies find the barriers initialised
         }
         __syncwarp();
-        for (uint32_t i = 0; i < head; ++i) {   // before the CTA is set up
+        asm volatile("bar.arrive 1, %0;" ::"n"(C::kThreads) : "memory");   // the barriers are there; nothing of the others is needed
+        for (uint32_t i = 0; i < head; ++i) {
             if (elected()) {
                 weights(k0 + i, i);
                 if (p.early != 1) tokens(k0 + i, i);
             }
             __syncwarp();
         }
+    } else {
+        if (warp == 1) {
+            tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
+            tmem_relinquish();
+        }
+        tc_fence_before();
+        asm volatile("bar.sync 1, %0;" ::"n"(C::kThreads) : "memory");
+        tc_fence_after();
     }
-    if (warp == 1) {
-        tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
-        tmem_relinquish();
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = tmem_slot, sfa = tmem + p.nt, sfb = sfa + 4 * C::kTiles;   // columns behind the accumulator
+    const uint32_t tmem = warp == 0 ? 0 : tmem_slot, sfa = tmem + p.nt, sfb = sfa + 4 * C::kTiles;   // columns behind the accumulator
     volatile int *abortp = &abort_flag;
 
+    // what the thread stores: four channels of every so many tokens, and their terms, fetched while the sums are made
+    const uint32_t tokens_here = min(p.nt, p.g.M - t0), c = (threadIdx.x & 31) * 4, n = tn * 128 + c;
+    uint16_t *out = reinterpret_cast<uint16_t *>(p.g.out);
+    const uint16_t *bias = reinterpret_cast<const uint16_t *>(p.g.bias);
+    const bool vec = (p.g.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0 && n + 4 <= p.g.N;
+    float f[4], b[4];
+    auto terms = [&] {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const bool in = n + j < p.g.N;
+            f[j] = in && p.g.w_rows ? __ldg(p.g.w_rows + n + j) : 1.f;
+            b[j] = in && bias ? Two<T>::up1(__ldg(bias + n + j)) : 0.f;
+        }
+    };
     if (warp == 0) {
         bool ok = true;
         if (p.early == 1) {
@@ -521,9 +540,11 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
         }
     } else {
+        terms();
         wait(acc_full, 0, abortp, 13);
         tc_fence_after();
     }
+    if (warp < 2) terms();
     if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens' factors
     if (warp >= 2 && !abort_flag) {
         const uint32_t quad = warp & 3, acc = tmem + ((quad * 32) << 16);
@@ -540,58 +561,64 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     // The partial sums of the cluster's CTAs meet in distributed shared memory; each CTA adds and stores a share of the
     // tokens, a token per warp and step and four channels per thread, always in the order of the CTAs. (Sent to the storing
     // CTA instead, 128 tokens, 4096 x 4096: 10.6 us against 9.4; 16 tokens: 6.8 against 7.2.)
-    const uint32_t tokens_here = min(p.nt, p.g.M - t0), c = (threadIdx.x & 31) * 4, n = tn * 128 + c;
-    uint16_t *out = reinterpret_cast<uint16_t *>(p.g.out);
-    const uint16_t *bias = reinterpret_cast<const uint16_t *>(p.g.bias);
-    const bool vec = (p.g.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0 && n + 4 <= p.g.N;
-    float f[4], b[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const bool in = n + j < p.g.N;
-        f[j] = in && p.g.w_rows ? __ldg(p.g.w_rows + n + j) : 1.f;
-        b[j] = in && bias ? Two<T>::up1(__ldg(bias + n + j)) : 0.f;
-    }
     if (p.splits > 1) cluster_barrier();
     else __syncthreads();
-    if (!abort_flag && n < p.g.N) {
-        for (uint32_t t = rank * (C::kThreads / 32) + warp; t < tokens_here; t += p.splits * (C::kThreads / 32)) {
-            const uint32_t m = t0 + t, local = smem_u32(part + t * 128 + c);
-            const float ra = p.g.a_rows ? p.g.a_rows[m] : 1.f;
-            float4 y;
-            if (p.splits == 1) {
-                y = *reinterpret_cast<const float4 *>(part + t * 128 + c);
-            } else {
-                float4 v[8];
-#pragma unroll
-                for (int s = 0; s < 8; ++s)
-                    if (s < p.splits)
-                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                                     : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w) : "r"(in_cta(local, s)));
-                y = v[0];
-#pragma unroll
-                for (int s = 1; s < 8; ++s)
-                    if (s < p.splits) { y.x += v[s].x; y.y += v[s].y; y.z += v[s].z; y.w += v[s].w; }
-            }
-            const uint2 w = make_uint2(Two<T>::down(finish(y.x, ra, f[0], b[0]), finish(y.y, ra, f[1], b[1])),
-                                       Two<T>::down(finish(y.z, ra, f[2], b[2]), finish(y.w, ra, f[3], b[3])));
-            uint16_t *o = out + (size_t)m * p.g.ldo + n;
-            if (vec) {
-                *reinterpret_cast<uint2 *>(o) = w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (n + j < p.g.N) o[j] = (uint16_t)((j < 2 ? w.x : w.y) >> (16 * (j & 1)));
-            }
-        }
-    }
-    if (p.splits > 1) cluster_barrier();   // the others have read this CTA's partial sums
-    else __syncthreads();
-    if (p.early == 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // this launch does not end before the one in front
-    if (warp == 1) {
-        __syncwarp();
+    if (warp == 1) {   // the accumulators have been read
         tc_fence_after();
         tmem_dealloc(tmem, p.tmem_cols);
     }
+    auto store = [&](uint32_t t, const float4 &y) {
+        const uint32_t m = t0 + t;
+        const float ra = p.g.a_rows ? p.g.a_rows[m] : 1.f;
+        const uint2 w = make_uint2(Two<T>::down(finish(y.x, ra, f[0], b[0]), finish(y.y, ra, f[1], b[1])),
+                                   Two<T>::down(finish(y.z, ra, f[2], b[2]), finish(y.w, ra, f[3], b[3])));
+        uint16_t *o = out + (size_t)m * p.g.ldo + n;
+        if (vec) {
+            *reinterpret_cast<uint2 *>(o) = w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < p.g.N) o[j] = (uint16_t)((j < 2 ? w.x : w.y) >> (16 * (j & 1)));
+        }
+    };
+    // U tokens at a time, so that their reads are on the way together
+    const uint32_t first = rank * (C::kThreads / 32) + warp, step = p.splits * (C::kThreads / 32);
+    auto gather = [&](auto us, auto splits) {
+        constexpr int U = decltype(us)::value, S = decltype(splits)::value;
+        for (uint32_t t = first; t < tokens_here; t += U * step) {
+            float4 v[U][S];
+#pragma unroll
+            for (int i = 0; i < U; ++i)
+#pragma unroll
+                for (int s = 0; s < S; ++s)
+                    if (t + i * step < tokens_here)
+                        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                                     : "=f"(v[i][s].x), "=f"(v[i][s].y), "=f"(v[i][s].z), "=f"(v[i][s].w)
+                                     : "r"(in_cta(smem_u32(part + (t + i * step) * 128 + c), s)));
+#pragma unroll
+            for (int i = 0; i < U; ++i) {
+                if (t + i * step >= tokens_here) break;
+                float4 y = v[i][0];
+#pragma unroll
+                for (int s = 1; s < S; ++s) { y.x += v[i][s].x; y.y += v[i][s].y; y.z += v[i][s].z; y.w += v[i][s].w; }
+                store(t + i * step, y);
+            }
+        }
+    };
+    if (!abort_flag && n < p.g.N) {
+        using std::integral_constant;
+        if (p.splits == 1) {
+            for (uint32_t t = first; t < tokens_here; t += step) store(t, *reinterpret_cast<const float4 *>(part + t * 128 + c));
+        } else if (p.splits == 2) {
+            gather(integral_constant<int, 4>{}, integral_constant<int, 2>{});
+        } else if (p.splits == 4) {
+            gather(integral_constant<int, 3>{}, integral_constant<int, 4>{});
+        } else {
+            gather(integral_constant<int, 1>{}, integral_constant<int, 8>{});
+        }
+    }
+    if (p.splits > 1) cluster_barrier();   // the others have read this CTA's partial sums
+    if (p.early == 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // this launch does not end before the one in front
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------
@@ -826,8 +853,8 @@ int duq4_linear_fp4_from_16bit(int format, int dtype, const void *x, const uint8
     rc = fp4_quantize_rows(format, dtype, x, M, K, K, codes, scales, rows, (cudaStream_t)stream);
     if (rc) return rc;
     const GemmArgs a{M, N, K, codes, scales, W, W_block_scales, rows, W_row_scales, bias, out, ldo};
-    // The product may start while the quantizer runs: the quantizer is an ordinary launch, so everything that was queued
-    // before it (the weights' upload among it) is done when it starts; what it writes itself is waited for in the kernel.
+    // The product may start while the quantizer runs: the quantizer lets it only when everything that was queued before (the
+    // weights' upload among it) is done; what the quantizer writes itself is waited for in the kernel.
     return run(format, dtype, a, (cudaStream_t)stream, true);
 }
 

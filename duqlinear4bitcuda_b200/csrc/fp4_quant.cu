@@ -2,6 +2,8 @@
 // product of a gate/up projection, and the residual sum between two blocks with its norms. One row kernel does all three:
 // a row is formed in registers, 16 neighbours per thread, and coded from there, so that no intermediate goes to memory.
 // No counterpart in the reference, whose quantizers are integer ones (qlinear4bit/nn/quantizer.py).
+#include <type_traits>
+
 #include "fp4_common.cuh"
 #include "quant_device.cuh"
 #include "trace_range.h"
@@ -208,8 +210,11 @@ __global__ void __maxnreg__(REGS) fp4_row_kernel(const RowArgs a) {
     const uint32_t chunks_all = a.cols >> 4, NT = LANES ? a.lanes : blockDim.x, tid = LANES ? threadIdx.x & (NT - 1) : threadIdx.x;
     const int lane = threadIdx.x & 31;
     const bool wide = a.wide != 0;
-    // a product launched behind the quantizer may start and fetch its weights (nothing happens without such a launch)
-    if (SRC == SRC_PLAIN) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // Few rows: this launch may begin while the one in front ends; it waits here, before its first access to memory. Only then may
+    // the next one begin (a product, which fetches its weights while these rows are coded): all that was queued earlier is
+    // done. Both do nothing in an ordinary launch.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // LANES: a warp's rows are neighbours; it goes on together until none of them exists
     const uint32_t per_warp = LANES ? 32 / NT : 1, mine = LANES ? lane / NT : 0;
     const uint32_t first = LANES ? (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * per_warp : blockIdx.x;
@@ -401,6 +406,8 @@ template <int FMT, class T>
 __global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
                                                           const float *__restrict__ row_scales, uint32_t rows, uint32_t cols,
                                                           T *__restrict__ out, bool wide) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t chunks = cols >> 4, tiles = scale_tiles(FMT, cols);
     const uint64_t total = (uint64_t)rows * chunks;
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
@@ -432,6 +439,26 @@ static bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintp
 
 // 16 neighbours per thread and chunk; rows of up to 65536 stay in registers.
 constexpr uint32_t kMaxCols = 65536;
+
+// A launch that may begin while the one in front on the stream ends (its kernel waits for that).
+template <class... P, class... A>
+static int launch_behind(uint32_t grid, uint32_t threads, cudaStream_t st, void (*kernel)(P...), A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();
+        return (int)e;
+    }
+    return launch_status();
+}
 
 template <int SRC, class T, int OUT>
 static int launch_rows(RowArgs a, cudaStream_t st) {
@@ -467,7 +494,7 @@ static int launch_rows(RowArgs a, cudaStream_t st) {
     // 41.1 / 40.9 / 38.9 / 39.0; norm joint 4096 x 11008, whose 352 threads fit twice with 64, three times with 48:
     // 88.1 / 79.6 / 78.0 / 105.8, but 2048 x 16384 56.4 / 60.8 / 60.4 / 82.4).
     if (a.rows < 296 && chunks <= 1024) {
-        fp4_row_kernel<SRC, T, OUT, 1, false, 64><<<grid, threads(1), 0, st>>>(a);
+        return launch_behind(grid, threads(1), st, fp4_row_kernel<SRC, T, OUT, 1, false, 64>, a);
     } else if (chunks <= kWide) {
         const uint32_t nt = threads(2);
         constexpr int kRegs = SRC == SRC_NORM ? 64 : OUT == OUT_MX ? 40 : SRC == SRC_SILU ? 48 : 64;
@@ -598,8 +625,15 @@ int duq4_fp4_dequantize(int format, int dtype, const uint8_t *codes, const uint8
     cudaStream_t st = (cudaStream_t)stream;
     const uint64_t total = (uint64_t)rows * (cols >> 4);
     const uint32_t grid = (uint32_t)((total + 255) / 256 < 148u * 32u ? (total + 255) / 256 : 148u * 32u);
+    int rc = DUQ4_OK;
     auto go = [&](auto fmt, auto *o) {
-        fp4_dequant_kernel<decltype(fmt)::value><<<grid, 256, 0, st>>>(codes, block_scales, row_scales, rows, cols, o, aligned(out, 32));
+        auto *kernel = fp4_dequant_kernel<decltype(fmt)::value, std::remove_pointer_t<decltype(o)>>;
+        if (grid < 296) {
+            rc = launch_behind(grid, 256, st, kernel, codes, block_scales, row_scales, rows, cols, o, aligned(out, 32));
+        } else {
+            kernel<<<grid, 256, 0, st>>>(codes, block_scales, row_scales, rows, cols, o, aligned(out, 32));
+            rc = launch_status();
+        }
     };
     auto by_type = [&](auto fmt) {
         if (dtype == DUQ4_DTYPE_F16) go(fmt, (__half *)out);
@@ -608,7 +642,7 @@ int duq4_fp4_dequantize(int format, int dtype, const uint8_t *codes, const uint8
     };
     if (format == kMX) by_type(std::integral_constant<int, kMX>{});
     else by_type(std::integral_constant<int, kNV>{});
-    return launch_status();
+    return rc;
 }
 
 }  // extern "C"
