@@ -25,6 +25,8 @@ __device__ int g_fp4_status = 0;
 int fp4_quantize_rows(int format, int dtype, const void *x, uint32_t rows, uint32_t cols, uint64_t ldx, uint8_t *codes, uint8_t *block_scales,
                       float *row_scales, cudaStream_t st);
 
+extern std::atomic<int> g_static_weights;   // duq4_set_static_weights
+
 namespace fp4 {
 
 using namespace ptx;
@@ -158,7 +160,6 @@ __device__ __forceinline__ void leave_copies_behind() {   // a producer that giv
 struct PairArgs {
     GemmArgs g;
     uint32_t tiles_m, tiles_n, bn;   // tiles of 256 tokens x bn channels (128 or 256)
-    uint32_t early;                  // 1: the tokens' quantizer is the launch in front and may still run
 };
 
 template <int FMT>
@@ -279,7 +280,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         tm = band * 16 + r % here;
     };
 
-    if (p.early) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the launch in front may still have run so far
     // the rest of the columns, where a second launch does them, may start: the tokens are there
     if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 0) {
@@ -406,7 +407,9 @@ struct SwapArgs {
     uint32_t nt, splits;     // tokens per tile (a multiple of 16; 128 where there are several tiles); CTAs that share a tile's K
     uint32_t tmem_cols;
     uint32_t stages;
-    uint32_t early;          // the launch in front may still run: 1: it is the tokens' quantizer, 2: nothing is needed of it
+    // What the launch in front, which may still run, leaves this one: 1: the weights are there (it is the tokens' quantizer, or the
+    // caller has promised so), 2: all is there, 3: nothing
+    uint32_t early;
 };
 
 template <int FMT>
@@ -438,7 +441,6 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     const uint32_t tn = blockIdx.x / p.splits, t0 = blockIdx.y * p.nt;
     const uint32_t ktiles = (p.g.K + kBK - 1) / kBK, k0 = rank * ktiles / p.splits, k1 = (rank + 1) * ktiles / p.splits;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the next launch on the stream may set itself up; it waits for this one
     const uint32_t head = min(p.stages, k1 - k0);   // the first round of stages
     auto weights = [&](uint32_t k, uint32_t s) {    // a stage's weights, and the bytes it waits for
         mbar_expect_tx(full(s), stage + 2 * C::kScale);
@@ -463,6 +465,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
         __syncwarp();
         asm volatile("bar.arrive 1, %0;" ::"n"(C::kThreads) : "memory");   // the barriers are there; nothing of the others is needed
+        if (p.early == 3) asm volatile("griddepcontrol.wait;" ::: "memory");
         for (uint32_t i = 0; i < head; ++i) {
             if (elected()) {
                 weights(k0 + i, i);
@@ -474,10 +477,13 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         if (warp == 1) {
             tmem_alloc(smem_u32(&tmem_slot), p.tmem_cols);
             tmem_relinquish();
+            // the next launch on the stream may set itself up (and take TMEM: not before this one has its own); it waits for this one
+            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         }
         tc_fence_before();
         asm volatile("bar.sync 1, %0;" ::"n"(C::kThreads) : "memory");
         tc_fence_after();
+        if (p.early == 3) asm volatile("griddepcontrol.wait;" ::: "memory");
     }
     const uint32_t tmem = warp == 0 ? 0 : tmem_slot, sfa = tmem + p.nt, sfb = sfa + 4 * C::kTiles;   // columns behind the accumulator
     volatile int *abortp = &abort_flag;
@@ -545,7 +551,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         tc_fence_after();
     }
     if (warp < 2) terms();
-    if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens' factors
+    if (p.early != 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens' factors, and whoever still reads the result
     if (warp >= 2 && !abort_flag) {
         const uint32_t quad = warp & 3, acc = tmem + ((quad * 32) << 16);
         for (uint32_t c = 0; c < p.nt; c += 16) {
@@ -654,7 +660,7 @@ static int map_scales(CUtensorMap *m, const uint8_t *p, int format, uint32_t row
 }
 
 template <class F>
-static int launch(F *kernel, uint32_t gx, uint32_t gy, uint32_t threads, uint32_t smem, uint32_t cluster, bool overlap, cudaStream_t st, const CUtensorMap (&maps)[4],
+static int launch(F *kernel, uint32_t gx, uint32_t gy, uint32_t threads, uint32_t smem, uint32_t cluster, cudaStream_t st, const CUtensorMap (&maps)[4],
                   const void *args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(gx, gy);
@@ -668,7 +674,7 @@ static int launch(F *kernel, uint32_t gx, uint32_t gy, uint32_t threads, uint32_
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = overlap ? 2 : 1;
+    cfg.numAttrs = 2;
     void *a[] = {(void *)&maps[0], (void *)&maps[1], (void *)&maps[2], (void *)&maps[3], const_cast<void *>(args)};
     const cudaError_t e = cudaLaunchKernelExC(&cfg, (const void *)kernel, a);
     if (e != cudaSuccess) {
@@ -679,7 +685,7 @@ static int launch(F *kernel, uint32_t gx, uint32_t gy, uint32_t threads, uint32_
 }
 
 template <int FMT, class T>
-static int launch_pair(const GemmArgs &g, cudaStream_t st, uint32_t early) {
+static int launch_pair(const GemmArgs &g, cudaStream_t st) {
     using C = Pair<FMT>;
     static DeviceOnce once;
     const int dev = current_device_slot();
@@ -687,7 +693,7 @@ static int launch_pair(const GemmArgs &g, cudaStream_t st, uint32_t early) {
     int rc = once.run(dev, [] { return (int)cudaFuncSetAttribute(fp4_pair_kernel<FMT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem); });
     if (rc) return rc;
     const uint32_t pairs = (uint32_t)sm_count_current_device() / 2;
-    PairArgs p{g, cdiv(g.M, 256), 0, 256, early};
+    PairArgs p{g, cdiv(g.M, 256), 0, 256};
     if ((uint64_t)p.tiles_m * cdiv(g.N, 256) * 2 <= pairs) p.bn = 128;
     p.tiles_n = cdiv(g.N, p.bn);
     CUtensorMap maps[4];
@@ -696,7 +702,7 @@ static int launch_pair(const GemmArgs &g, cudaStream_t st, uint32_t early) {
         return rc;
     if ((uint64_t)p.tiles_m * p.tiles_n > 0x7FFFFFFFull) return DUQ4_ERR_SHAPE;
     const uint32_t n = p.tiles_m * p.tiles_n < pairs ? p.tiles_m * p.tiles_n : pairs;
-    return launch(fp4_pair_kernel<FMT, T>, 2 * n, 1, C::kThreads, C::kSmem, 2, early != 0, st, maps, &p);
+    return launch(fp4_pair_kernel<FMT, T>, 2 * n, 1, C::kThreads, C::kSmem, 2, st, maps, &p);
 }
 
 // CTAs that share a tile's K: up to eight while there is an SM for each (M 16, 4096 x 4096: 9.0 / 8.3 / 7.5 / 7.6 us with 1 / 2 / 4 /
@@ -739,7 +745,7 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, uint32_t early) {
     if ((rc = map_codes(&maps[0], g.a, g.M, g.K, p.nt)) || (rc = map_codes(&maps[1], g.w, g.N, g.K, 128)) ||
         (rc = map_scales(&maps[2], g.a_scales, FMT, g.M, g.K, 1)) || (rc = map_scales(&maps[3], g.w_scales, FMT, g.N, g.K, 1)))
         return rc;
-    return launch(fp4_swap_kernel<FMT, T>, tiles_n * p.splits, tiles_m, C::kThreads, smem, p.splits, early != 0, st, maps, &p);
+    return launch(fp4_swap_kernel<FMT, T>, tiles_n * p.splits, tiles_m, C::kThreads, smem, p.splits, st, maps, &p);
 }
 
 // Which kernel. Both are priced in 10 ns by the columns of K that the busiest SM goes through, in steps of 256: 0.37 us for the
@@ -753,12 +759,12 @@ static uint64_t swap_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
     return (tiles * splits + sms - 1) / sms * ((ktiles + splits - 1) / splits) * 45 + 200;
 }
 template <int FMT, class T>
-static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
-    if (a.M <= 128) return launch_swap<FMT, T>(a, st, overlap);
+static int gemm(const GemmArgs &a, cudaStream_t st, uint32_t early) {
+    if (a.M <= 128) return launch_swap<FMT, T>(a, st, early);
     const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK), tiles_m = cdiv(a.M, 256), tiles_n = cdiv(a.N, 256);
     const uint64_t all = pair_price(tiles_m * tiles_n, ktiles, sms), blocks_m = cdiv(a.M, 128);
     const bool swap_fits = blocks_m <= 65535;   // the grid's second dimension
-    if (swap_fits && swap_price(blocks_m * cdiv(a.N, 128), ktiles, sms) < all) return launch_swap<FMT, T>(a, st, overlap);
+    if (swap_fits && swap_price(blocks_m * cdiv(a.N, 128), ktiles, sms) < all) return launch_swap<FMT, T>(a, st, early);
     // A last round that few tiles are left for: whole rounds by the pair kernel, the columns that are left by the other one,
     // launched behind it (512 x 28672 x 8192, 3 rounds and 2 tiles of 256 x 256: 57.9 -> 53.3 us).
     const uint64_t rest = tiles_m * tiles_n % (sms / 2), strip = rest ? (rest + tiles_m - 1) / tiles_m : 0;
@@ -774,11 +780,11 @@ static int gemm(const GemmArgs &a, cudaStream_t st, bool overlap) {
             if (a.w_rows) left.w_rows += n0;
             if (a.bias) left.bias = reinterpret_cast<const uint16_t *>(a.bias) + n0;
             left.out = reinterpret_cast<uint16_t *>(a.out) + n0;
-            const int rc = launch_pair<FMT, T>(main, st, overlap);
+            const int rc = launch_pair<FMT, T>(main, st);
             return rc ? rc : launch_swap<FMT, T>(left, st, 2);
         }
     }
-    return launch_pair<FMT, T>(a, st, overlap);
+    return launch_pair<FMT, T>(a, st);
 }
 
 static int check_gemm(int format, int dtype, uint32_t M, uint32_t N, uint32_t K, uint64_t ldo) {
@@ -789,9 +795,9 @@ static int check_gemm(int format, int dtype, uint32_t M, uint32_t N, uint32_t K,
 }
 static bool aligned(const void *p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
-static int run(int format, int dtype, const GemmArgs &a, cudaStream_t st, bool overlap) {
-    if (format == kMX) return dtype == DUQ4_DTYPE_F16 ? gemm<kMX, __half>(a, st, overlap) : gemm<kMX, __nv_bfloat16>(a, st, overlap);
-    return dtype == DUQ4_DTYPE_F16 ? gemm<kNV, __half>(a, st, overlap) : gemm<kNV, __nv_bfloat16>(a, st, overlap);
+static int run(int format, int dtype, const GemmArgs &a, cudaStream_t st, uint32_t early) {
+    if (format == kMX) return dtype == DUQ4_DTYPE_F16 ? gemm<kMX, __half>(a, st, early) : gemm<kMX, __nv_bfloat16>(a, st, early);
+    return dtype == DUQ4_DTYPE_F16 ? gemm<kNV, __half>(a, st, early) : gemm<kNV, __nv_bfloat16>(a, st, early);
 }
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -830,7 +836,7 @@ int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales,
         !aligned(W_row_scales, 4) || !aligned(bias, 2) || !aligned(out, 2))
         return DUQ4_ERR_ALIGN;
     const GemmArgs a{M, N, K, A, A_block_scales, W, W_block_scales, A_row_scales, W_row_scales, bias, out, ldo};
-    return run(format, dtype, a, (cudaStream_t)stream, false);
+    return run(format, dtype, a, (cudaStream_t)stream, g_static_weights.load(std::memory_order_relaxed) ? 1 : 3);
 }
 
 size_t duq4_linear_fp4_workspace_bytes(int format, uint32_t M, uint32_t K) {
@@ -855,7 +861,7 @@ int duq4_linear_fp4_from_16bit(int format, int dtype, const void *x, const uint8
     const GemmArgs a{M, N, K, codes, scales, W, W_block_scales, rows, W_row_scales, bias, out, ldo};
     // The product may start while the quantizer runs: the quantizer lets it only when everything that was queued before (the
     // weights' upload among it) is done; what the quantizer writes itself is waited for in the kernel.
-    return run(format, dtype, a, (cudaStream_t)stream, true);
+    return run(format, dtype, a, (cudaStream_t)stream, 1);
 }
 
 }  // extern "C"

@@ -210,9 +210,8 @@ __global__ void __maxnreg__(REGS) fp4_row_kernel(const RowArgs a) {
     const uint32_t chunks_all = a.cols >> 4, NT = LANES ? a.lanes : blockDim.x, tid = LANES ? threadIdx.x & (NT - 1) : threadIdx.x;
     const int lane = threadIdx.x & 31;
     const bool wide = a.wide != 0;
-    // Few rows: this launch may begin while the one in front ends; it waits here, before its first access to memory. Only then may
-    // the next one begin (a product, which fetches its weights while these rows are coded): all that was queued earlier is
-    // done. Both do nothing in an ordinary launch.
+    // This launch may begin while the one in front ends; it waits here, before its first access to memory. Only then may the
+    // next one begin (a product, which fetches its weights while these rows are coded): all that was queued earlier is done.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     // LANES: a warp's rows are neighbours; it goes on together until none of them exists
@@ -485,8 +484,7 @@ static int launch_rows(RowArgs a, cudaStream_t st) {
         if (chunks <= 32 && a.rows >= 296) {
             a.lanes = chunks <= 8 ? 8 : chunks <= 16 ? 16 : 32;
             const uint64_t blocks = ((uint64_t)a.rows * a.lanes + 255) / 256;
-            fp4_row_kernel<SRC, T, OUT, 1, true, 64><<<blocks < 148u * 64u ? (uint32_t)blocks : 148u * 64u, 256, 0, st>>>(a);
-            return launch_status();
+            return launch_behind(blocks < 148u * 64u ? (uint32_t)blocks : 148u * 64u, 256, st, fp4_row_kernel<SRC, T, OUT, 1, true, 64>, a);
         }
     }
     // Registers a thread may have: fewer where that puts more rows on an SM at little spilling (us with 64 / 56 / 48 / 40 at
@@ -498,12 +496,10 @@ static int launch_rows(RowArgs a, cudaStream_t st) {
     } else if (chunks <= kWide) {
         const uint32_t nt = threads(2);
         constexpr int kRegs = SRC == SRC_NORM ? 64 : OUT == OUT_MX ? 40 : SRC == SRC_SILU ? 48 : 64;
-        if (SRC == SRC_NORM && 1024 / nt * nt < 768) fp4_row_kernel<SRC, T, OUT, 2, false, SRC == SRC_NORM ? 48 : kRegs><<<grid, nt, 0, st>>>(a);
-        else fp4_row_kernel<SRC, T, OUT, 2, false, kRegs><<<grid, nt, 0, st>>>(a);
-    } else {
-        fp4_row_kernel<SRC, T, OUT, 4, false, 64><<<grid, threads(4), 0, st>>>(a);
+        if (SRC == SRC_NORM && 1024 / nt * nt < 768) return launch_behind(grid, nt, st, fp4_row_kernel<SRC, T, OUT, 2, false, SRC == SRC_NORM ? 48 : kRegs>, a);
+        return launch_behind(grid, nt, st, fp4_row_kernel<SRC, T, OUT, 2, false, kRegs>, a);
     }
-    return launch_status();
+    return launch_behind(grid, threads(4), st, fp4_row_kernel<SRC, T, OUT, 4, false, 64>, a);
 }
 
 static int check_fp4(int format, int dtype, uint32_t cols) {
@@ -628,12 +624,7 @@ int duq4_fp4_dequantize(int format, int dtype, const uint8_t *codes, const uint8
     int rc = DUQ4_OK;
     auto go = [&](auto fmt, auto *o) {
         auto *kernel = fp4_dequant_kernel<decltype(fmt)::value, std::remove_pointer_t<decltype(o)>>;
-        if (grid < 296) {
-            rc = launch_behind(grid, 256, st, kernel, codes, block_scales, row_scales, rows, cols, o, aligned(out, 32));
-        } else {
-            kernel<<<grid, 256, 0, st>>>(codes, block_scales, row_scales, rows, cols, o, aligned(out, 32));
-            rc = launch_status();
-        }
+        rc = launch_behind(grid, 256, st, kernel, codes, block_scales, row_scales, rows, cols, o, aligned(out, 32));
     };
     auto by_type = [&](auto fmt) {
         if (dtype == DUQ4_DTYPE_F16) go(fmt, (__half *)out);

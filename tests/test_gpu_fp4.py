@@ -615,3 +615,50 @@ def test_norm_into_the_integer_layers(fmt, rows, cols):
         lin = nn.Linear4bitSQ(cols, 64).cuda()
         lin.weight_scales.fill_(0.01)
         assert torch.equal(lin(q), lin(want))
+
+
+@pytest.mark.parametrize("static", [0, 1])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_long_chain_of_launches_keeps_its_order(fmt, static):
+    """Launches that overlap the ones in front: a chain in which every call reads what the call before wrote, buffers reused all the
+    time, integer layers and plain torch kernels between; with and without the promise on weights. As the same chain with a
+    wait after every call."""
+    import duqlinear4bitcuda_b200.lib as L
+    import duqlinear4bitcuda_b200.nn as nn
+    g = torch.Generator().manual_seed(1)
+    dim, dtype = 512, torch.float16
+    lin = lambda i, o: torch.nn.Linear(i, o, bias=True).to(dtype).cuda()
+    up, down = nn.LinearFP4.from_linear(lin(dim, 2 * dim), fmt, dtype), nn.LinearFP4.from_linear(lin(dim, dim), fmt, dtype)
+    tall = nn.LinearFP4.from_linear(lin(dim, 20000), fmt, dtype)
+    integer = nn.Linear4bitASQ(dim, dim).cuda()
+    integer.weight_scales.fill_(0.05)
+    joint, glue = nn.NormResidualQuantizer(dim, fmt, post_norm=True, residual_scale=0.5, dtype=dtype).cuda(), nn.SiluMulQuantizerFP4(fmt)
+
+    def chain(x, wait):
+        stream = x
+        for i in range(12):
+            for f in ((lambda t: up(t)), (lambda t: glue(t)), (lambda t: down(t))):
+                x = f(x)
+                if wait:
+                    torch.cuda.synchronize()
+            q, stream = joint(x, stream)
+            x = q.dequantize(dtype)
+            if wait:
+                torch.cuda.synchronize()
+            x = integer(x) * 0.5 if i % 3 == 0 else x + 0.25
+            if i % 4 == 0:
+                x = x + tall(x)[:, 7:7 + dim] * 0.1
+            if wait:
+                torch.cuda.synchronize()
+            x = x.clamp(-8, 8)
+        return x, stream
+    old = L.cdll.duq4_set_static_weights(static)
+    try:
+        for tokens in (1, 17, 140, 700):
+            x = torch.randn(tokens, dim, generator=g).to(dtype).cuda()
+            want = chain(x, True)
+            for _ in range(3):
+                got = chain(x, False)
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    finally:
+        L.cdll.duq4_set_static_weights(old)
