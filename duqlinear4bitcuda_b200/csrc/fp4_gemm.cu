@@ -498,8 +498,9 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const bool in = n + j < p.g.N;
-            f[j] = in && p.g.w_rows ? __ldg(p.g.w_rows + n + j) : 1.f;
-            b[j] = in && bias ? Two<T>::up1(__ldg(bias + n + j)) : 0.f;
+            // plain loads: read-only-path ones may be moved ahead of a wait
+            f[j] = in && p.g.w_rows ? p.g.w_rows[n + j] : 1.f;
+            b[j] = in && bias ? Two<T>::up1(bias[n + j]) : 0.f;
         }
     };
     if (warp == 0) {
@@ -523,6 +524,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
         if (!ok) leave_copies_behind();
     } else if (warp == 1) {
+        if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");   // the launch in front may take longer than a wait on a barrier may
         bool ok = true, issued = false;
         const uint32_t idesc = block_idesc<FMT>(128, p.nt);
         const uint64_t desc_w = make_desc(base), desc_s = scale_desc(scales0);
@@ -547,11 +549,13 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
     } else {
         terms();
+        if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");
         wait(acc_full, 0, abortp, 13);
         tc_fence_after();
     }
     if (warp < 2) terms();
-    if (p.early != 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // the tokens' factors, and whoever still reads the result
+    // From here on the tokens' factors are read and the result is written: unless all is there from the start, every warp has
+    // waited for the launch in front.
     if (warp >= 2 && !abort_flag) {
         const uint32_t quad = warp & 3, acc = tmem + ((quad * 32) << 16);
         for (uint32_t c = 0; c < p.nt; c += 16) {

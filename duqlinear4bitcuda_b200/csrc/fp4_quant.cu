@@ -400,11 +400,11 @@ __global__ void __maxnreg__(REGS) fp4_row_kernel(const RowArgs a) {
     }
 }
 
-// Codes back to values: code * (block scale * row scale), rounded once. One thread per 16 neighbours.
+// Codes back to values: code * (block scale * row scale), rounded once. One thread per 16 neighbours. (No read-only-path
+// loads, which need not stay behind the wait.)
 template <int FMT, class T>
-__global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                                                          const float *__restrict__ row_scales, uint32_t rows, uint32_t cols,
-                                                          T *__restrict__ out, bool wide) {
+__global__ void __launch_bounds__(256) fp4_dequant_kernel(const uint8_t *codes, const uint8_t *scales, const float *row_scales, uint32_t rows,
+                                                          uint32_t cols, T *out, bool wide) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t chunks = cols >> 4, tiles = scale_tiles(FMT, cols);
