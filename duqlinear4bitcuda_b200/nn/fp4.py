@@ -17,7 +17,7 @@ def _check_format(format):
 
 def _packed(format, parts, lead, dtype):
     codes, block_scales, row_scales = parts
-    return PackedFP4Tensor(format, codes.view(*lead, -1), block_scales, row_scales, dtype)
+    return PackedFP4Tensor(format, codes.view(*lead, codes.shape[1]), block_scales, row_scales, dtype)
 
 
 class QuantizerFP4(torch.nn.Module):
@@ -77,14 +77,14 @@ class NormResidualQuantizer(torch.nn.Module):
                 gate = _as_rows(gate)[0]
         stream, *q = ops.norm_residual_quantize(self.format, x2, self.weight, self.eps, residual, post, gate, self.residual_scale)
         if self.format == "none":
-            out = q[0].view(*lead, -1)
+            out = q[0].view(x.shape)
         elif self.format == "sym":
-            out = PackedQuantizedTensor(q[0].view(*lead, -1), q[1].view(_scale_shape(lead)))
+            out = PackedQuantizedTensor(q[0].view(*lead, q[0].shape[1]), q[1].view(_scale_shape(lead)))
         elif self.format == "asym":
-            out = PackedQuantizedTensor(q[0].view(*lead, -1), q[1].view(*lead, 1), q[2].view(*lead, 1))
+            out = PackedQuantizedTensor(q[0].view(*lead, q[0].shape[1]), q[1].view(*lead, 1), q[2].view(*lead, 1))
         else:
             out = _packed(self.format, q, lead, x.dtype)
-        return out if residual is None else (out, stream.view(*lead, -1))
+        return out if residual is None else (out, stream.view(x.shape))
 
 
 class LinearFP4(torch.nn.Module):
@@ -120,7 +120,7 @@ class LinearFP4(torch.nn.Module):
         else:
             x2, lead = _as_rows(x)
             y = ops.linear_fp4_from_16bit(self.format, x2, *w, self.bias)
-        return y.view(*lead, -1)
+        return y.view(*lead, self.out_features)
 
     @classmethod
     def from_linear(cls, module: torch.nn.Linear, format="nvfp4", dtype=torch.float16):

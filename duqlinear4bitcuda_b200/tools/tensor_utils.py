@@ -49,7 +49,7 @@ class PackedFP4Tensor:
     def dequantize(self, dtype=None):
         """The values, [..., K]."""
         v = ops.fp4_dequantize(self.format, _rows(self.codes)[0], self.block_scales, self.row_scales, self.dtype if dtype is None else dtype)
-        return v.view(*self.codes.shape[:-1], -1)
+        return v.view(*self.codes.shape[:-1], v.shape[1])
 
 
 def _rows(t):

@@ -259,6 +259,25 @@ def test_empty_batches():
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lead", [(0,), (2, 0), (0, 3)])
+def test_modules_on_empty_batches(fmt, lead):
+    import duqlinear4bitcuda_b200.nn as nn
+    x = torch.empty(*lead, 64, dtype=torch.float16, device="cuda")
+    layer = nn.LinearFP4.from_linear(torch.nn.Linear(64, 40, bias=True).half().cuda(), fmt)
+    q = nn.QuantizerFP4(fmt)(x)
+    assert q.size() == (*lead, 32) and q.dequantize().shape == x.shape
+    assert layer(x).shape == (*lead, 40) and layer(q).shape == (*lead, 40)
+    assert nn.SiluMulQuantizerFP4(fmt)(x).size() == (*lead, 16)
+    for form in (fmt, "sym", "asym", "none"):
+        out, stream = nn.NormResidualQuantizer(64, form, post_norm=True).cuda()(x, x, x)
+        assert stream.shape == x.shape
+        if form == "none":
+            assert out.shape == x.shape
+        else:
+            assert out.size() == (*lead, 32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("tokens", [1, 19, 300])
 def test_mlp_block_of_modules(fmt, tokens):
     """The operators as they are used: norm -> gate/up layer -> SiLU product -> down layer -> norm after the block, residual
