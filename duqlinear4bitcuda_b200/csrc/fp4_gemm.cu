@@ -709,11 +709,13 @@ static int launch_pair(const GemmArgs &g, cudaStream_t st) {
     return launch(fp4_pair_kernel<FMT, T>, 2 * n, 1, C::kThreads, C::kSmem, 2, st, maps, &p);
 }
 
-// CTAs that share a tile's K: up to eight while there is an SM for each (M 16, 4096 x 4096: 9.0 / 8.3 / 7.5 / 7.6 us with 1 / 2 / 4 /
-// 8; 22016 x 4096, 172 tiles: 13.1 / 17.5 us with 1 / 2, whose 344 CTAs do not fit at once).
-static uint32_t swap_splits(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
+// CTAs that share a tile's K: up to eight while there is an SM for each (nvfp4, us with 1 / 2 / 4 / 8: 16 tokens, 4096 x 4096 6.5 /
+// 5.7 / 5.5 / 6.3; 1024 x 11008 12.0 / 8.1 / 5.7 / 5.3; 22016 x 4096, 172 tiles: 12.2 / 14.8, whose 344 CTAs do not fit at once).
+// With more than 64 tokens the partial sums weigh more: beyond two CTAs, each keeps a step of K for every four tiles (128 tokens:
+// 4096 x 4096, 32 tiles, 10.2 / 8.4 / 9.4; 2048 x 2048, 16 tiles, 7.8 / 6.8 / 7.0 / 7.4; 2048 x 11008 16.6 / 11.5 / 10.9 / 10.3).
+static uint32_t swap_splits(uint32_t M, uint64_t tiles, uint64_t ktiles, uint64_t sms) {
     uint32_t splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= sms && ktiles >= splits * 2) splits *= 2;
+    while (splits < 8 && tiles * splits * 2 <= sms && ktiles >= splits * 2 && (M <= 64 || splits == 1 || ktiles * 4 >= splits * 2 * tiles)) splits *= 2;
     return splits;
 }
 template <int FMT, class T>
@@ -732,7 +734,7 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, uint32_t early) {
     p.tmem_cols = cols <= 64 ? 64 : cols <= 128 ? 128 : 256;
     const uint32_t per_stage = C::stage_bytes(p.nt) + 2 * C::kScale;
     const uint32_t sms = (uint32_t)sm_count_current_device();
-    p.splits = swap_splits((uint64_t)tiles_n * tiles_m, ktiles, sms);
+    p.splits = swap_splits(g.M, (uint64_t)tiles_n * tiles_m, ktiles, sms);
     // stages: an SM's shared memory for one CTA, or half of it (228 KiB, 1 KiB a CTA taken) for two
     const bool alone = p.splits <= 2 && (uint64_t)tiles_n * tiles_m * p.splits <= sms;   // (wider clusters pack badly one CTA to an SM)
     p.stages = ((alone ? 220 : 111) * 1024) / per_stage;
@@ -752,30 +754,34 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, uint32_t early) {
     return launch(fp4_swap_kernel<FMT, T>, tiles_n * p.splits, tiles_m, C::kThreads, smem, p.splits, st, maps, &p);
 }
 
-// Which kernel. Both are priced in 10 ns by the columns of K that the busiest SM goes through, in steps of 256: 0.37 us for the
-// pair kernel's 256 x 256 (cold weights; a tile's epilogue hides behind the next tile), 0.45 us for the other one's
-// 128 x 128 with all SMs at work, and 2 us for its meeting. (Measured, nvfp4, pair / swap, us: 128 tokens x 22016 x 4096
-// 21.5 / 17.1; 256 x 22016 x 4096 21.5 / 29.1; 256 x 4096 x 11008 19.9 / 15.9; 512 x 4096 x 4096 11.0 / 13.8;
-// 4149 x 45 x 24800 36.7 / 16.8; 1024 x 1024 x 1024 6.8 / 8.7.)
-static uint64_t pair_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) { return (tiles + sms / 2 - 1) / (sms / 2) * ktiles * 37; }
-static uint64_t swap_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
-    const uint64_t splits = swap_splits(tiles, ktiles, sms);
-    return (tiles * splits + sms - 1) / sms * ((ktiles + splits - 1) / splits) * 45 + 200;
+// Which kernel. Both are priced by the columns of K that the busiest SM goes through, in steps of 256, and a fixed part: for the
+// pair kernel with tiles of 256 x 256 or, where those leave half of the pairs idle, 256 x 128; for the other one without and with
+// a meeting. The numbers are relative: fitted to both kernels' times at 234 sizes (144 .. 2048 tokens, 1024 .. 28672 channels, K
+// 2048 .. 11008, both formats) so that the cheapest is the fastest; what they choose is at most 4 % slower than the best choice at
+// any of those. (Measured, nvfp4, pair / swap / whole rounds and rest, us: 256 x 22016 x 4096 18.2 / 25.8 / 21.4; 256 x 4096 x
+// 11008 14.9 / 13.1; 300 x 11008 x 4096 16.4 / 14.9 / 19.3; 512 x 4096 x 4096 9.3 / 11.0; 4149 x 45 x 24800 32.7 / 20.7;
+// 512 x 28672 x 8192 55.2 / 96.2 / 54.0.)
+static uint64_t pair_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
+    return tiles * 4 <= sms ? ktiles * 50 + 140 : (tiles + sms / 2 - 1) / (sms / 2) * ktiles * 63 + 750;
+}
+static uint64_t swap_price(uint32_t M, uint64_t tiles, uint64_t ktiles, uint64_t sms) {
+    const uint64_t splits = swap_splits(M, tiles, ktiles, sms);
+    return (tiles * splits + sms - 1) / sms * ((ktiles + splits - 1) / splits) * 50 + (splits > 1 ? 1120 : 810);
 }
 template <int FMT, class T>
 static int gemm(const GemmArgs &a, cudaStream_t st, uint32_t early) {
     if (a.M <= 128) return launch_swap<FMT, T>(a, st, early);
     const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK), tiles_m = cdiv(a.M, 256), tiles_n = cdiv(a.N, 256);
-    const uint64_t all = pair_price(tiles_m * tiles_n, ktiles, sms), blocks_m = cdiv(a.M, 128);
+    const uint64_t blocks_m = cdiv(a.M, 128), pairs = pair_price(tiles_m * tiles_n, ktiles, sms);
     const bool swap_fits = blocks_m <= 65535;   // the grid's second dimension
-    if (swap_fits && swap_price(blocks_m * cdiv(a.N, 128), ktiles, sms) < all) return launch_swap<FMT, T>(a, st, early);
+    const uint64_t swap = swap_fits ? swap_price(a.M, blocks_m * cdiv(a.N, 128), ktiles, sms) : ~0ull, one = swap < pairs ? swap : pairs;
     // A last round that few tiles are left for: whole rounds by the pair kernel, the columns that are left by the other one,
-    // launched behind it (512 x 28672 x 8192, 3 rounds and 2 tiles of 256 x 256: 57.9 -> 53.3 us).
+    // launched behind it (512 x 28672 x 8192, 3 rounds and 2 tiles of 256 x 256).
     const uint64_t rest = tiles_m * tiles_n % (sms / 2), strip = rest ? (rest + tiles_m - 1) / tiles_m : 0;
     if (swap_fits && strip && strip < tiles_n) {
         const uint32_t n0 = (uint32_t)(tiles_n - strip) * 256;
-        const uint64_t both = pair_price(tiles_m * (tiles_n - strip), ktiles, sms) + swap_price(blocks_m * cdiv(a.N - n0, 128), ktiles, sms);
-        if (both < all) {
+        const uint64_t both = pair_price(tiles_m * (tiles_n - strip), ktiles, sms) + swap_price(a.M, blocks_m * cdiv(a.N - n0, 128), ktiles, sms) + 160;
+        if (both < one) {
             GemmArgs main = a, left = a;
             main.N = n0;
             left.N = a.N - n0;
@@ -788,7 +794,7 @@ static int gemm(const GemmArgs &a, cudaStream_t st, uint32_t early) {
             return rc ? rc : launch_swap<FMT, T>(left, st, 2);
         }
     }
-    return launch_pair<FMT, T>(a, st);
+    return swap < pairs ? launch_swap<FMT, T>(a, st, early) : launch_pair<FMT, T>(a, st);
 }
 
 static int check_gemm(int format, int dtype, uint32_t M, uint32_t N, uint32_t K, uint64_t ldo) {
