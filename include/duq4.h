@@ -75,7 +75,8 @@ int duq4_tensor_map_cache_entries(void);
  * are parameters, uploaded and synchronised before use). The small-M (M <= 16) kernels are then
  * launched with programmatic stream serialization and start streaming weights and per-channel
  * vectors while the preceding kernel of the stream is still finishing; activations, per-token
- * scales and all outputs still wait for it. Off by default (full stream ordering). Returns the
+ * scales and all outputs still wait for it. duq4_linear_fp4 with few tokens honours it the same way
+ * (its W, W_block_scales, W_row_scales and bias). Off by default (full stream ordering). Returns the
  * previous value. No reference counterpart. */
 int duq4_set_static_weights(int on);
 
@@ -479,7 +480,10 @@ int duq4_reduce_dequant_gather(const int32_t *slabs, uint32_t n_slabs, uint32_t 
  * of a tile at byte 16 * (r % 32) + 4 * (r / 32), the tiles of a block of rows one behind the other;
  * duq4_fp4_scale_bytes bytes in all. Scale bytes of columns beyond the row's end must be 0 (the quantizers write them so);
  * those of rows beyond the last one are not read into any result and are left as they were.
- * cols / K % 32 == 0; the quantizers take rows of up to 65536 columns. 16-bit tensors are fp16 or bfloat16 (`dtype`). */
+ * cols / K % 32 == 0; the quantizers take rows of up to 65536 columns. 16-bit tensors are fp16 or bfloat16 (`dtype`).
+ * The kernels are launched with programmatic stream serialization: they may become resident while the stream's launch in
+ * front still runs, and wait for its end before their first access to memory (weights excepted, where
+ * duq4_set_static_weights allows it). */
 #define DUQ4_FP4_MX 16
 #define DUQ4_FP4_NV 17
 #define DUQ4_DTYPE_F16 0

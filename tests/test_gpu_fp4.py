@@ -357,6 +357,35 @@ def test_linear_whole_rounds_and_a_rest(fmt, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("form", ["plain", "bias and strides"])
+def test_linear_a_rest_worth_a_second_launch(fmt, form):
+    """Long rows and few tiles behind the whole rounds: the columns that are left are another kernel's launch. Columns on both sides
+    of the seam, the last ones, and rows that are farther apart than they are long, against the definition."""
+    import duqlinear4bitcuda_b200.lib as L
+    m, n, k, dtype = 1000, 4994, 8224, torch.bfloat16
+    ap, at, ar, av = F.random_operand(fmt, m, k, 1)
+    wp, wt, wr, wv = F.random_operand(fmt, n, k, 2)
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(3)).to(dtype) if form != "plain" else None
+    a, w = [F.cuda(t) for t in (ap, at, ar)], [F.cuda(t) for t in (wp, wt, wr)]
+    if bias is None:
+        got = ops().linear_fp4(fmt, *a, *w, None, dtype)
+    else:
+        bias = bias.cuda()
+        ld = n + 3
+        room = torch.full((m, ld), 77.0, dtype=dtype, device="cuda")
+        ptr = lambda t: t.data_ptr()
+        assert L.cdll.duq4_linear_fp4(L.FP4_MX if fmt == "mxfp4" else L.FP4_NV, *map(ptr, a), *map(ptr, w), m, n, k, ptr(bias), L.DTYPE_BF16, ptr(room), ld,
+                                      torch.cuda.current_stream().cuda_stream) == 0
+        assert (room[:, n:] == 77).all()
+        got = room[:, :n]
+    b64 = None if bias is None else bias.double().cpu().numpy()
+    rows = [0, 1, 127, 128, 255, 256, 767, 768, 998, 999]
+    check_product(got[rows], av[rows], wv, b64, dtype)
+    cols = sorted(set(range(0, n, 256)) | set(range(255, n, 256)) | {n - 1})
+    check_product(got[:, cols], av, wv[cols], None if b64 is None else b64[cols], dtype)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rows,cols", [(20000, 96), (5000, 1056), (1500, 8192), (700, 16416), (400, 28672), (160, 65536)])
 def test_many_rows(fmt, rows, cols):
     """More rows than CTAs fit, so that a CTA does several: the first, the last and some between against the definition, the SiLU
