@@ -757,8 +757,8 @@ static int launch_swap(const GemmArgs &g, cudaStream_t st, uint32_t early) {
 // Which kernel. Both are priced by the columns of K that the busiest SM goes through, in steps of 256, and a fixed part: for the
 // pair kernel with tiles of 256 x 256 or, where those leave half of the pairs idle, 256 x 128; for the other one without and with
 // a meeting. The numbers are relative: fitted to both kernels' times at 234 sizes (144 .. 2048 tokens, 1024 .. 28672 channels, K
-// 2048 .. 11008, both formats) so that the cheapest is the fastest; what they choose is at most 4 % slower than the best choice at
-// any of those. (Measured, nvfp4, pair / swap / whole rounds and rest, us: 256 x 22016 x 4096 18.2 / 25.8 / 21.4; 256 x 4096 x
+// 2048 .. 11008, both formats) so that the cheapest is the fastest; in the fit what they choose is at most
+// 4 % slower than the best choice. (Measured, nvfp4, pair / swap / whole rounds and rest, us: 256 x 22016 x 4096 18.2 / 25.8 / 21.4; 256 x 4096 x
 // 11008 14.9 / 13.1; 300 x 11008 x 4096 16.4 / 14.9 / 19.3; 512 x 4096 x 4096 9.3 / 11.0; 4149 x 45 x 24800 32.7 / 20.7;
 // 512 x 28672 x 8192 55.2 / 96.2 / 54.0.)
 static uint64_t pair_price(uint64_t tiles, uint64_t ktiles, uint64_t sms) {
