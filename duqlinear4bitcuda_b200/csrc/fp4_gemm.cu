@@ -151,7 +151,9 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap *map, ui
     else
         tma_load_3d(dst, map, bar, x, y, z);
 }
-__device__ __forceinline__ void leave_copies_behind() {   // a producer that gives up lets its copies land first
+// A CTA in which a wait ran out lets its copies land before it gives its shared memory back. Called behind a barrier of the CTA, so
+// that it does not matter which warp gave up: the one that consumes may, when the producer has long issued its last copy.
+__device__ __forceinline__ void leave_copies_behind() {
     const uint64_t t0 = globaltimer();
     while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
 }
@@ -304,7 +306,6 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (++s == C::kStages) { s = 0; ph ^= 1; }
             }
         }
-        if (!ok) leave_copies_behind();
     } else if (warp == 1) {
         if (rank == 0) {
             uint32_t s = 0, ph = 0, lt = 0;
@@ -393,6 +394,8 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
+    if (abort_flag && warp == 0) leave_copies_behind();   // whichever wait ran out; before the partner's memory may go
+    __syncwarp();
     cluster_barrier();   // the partner is done with this CTA's shared memory and TMEM
     if (warp == 1) {
         __syncwarp();
@@ -504,7 +507,6 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
     };
     if (warp == 0) {
-        bool ok = true;
         if (p.early == 1) {
             asm volatile("griddepcontrol.wait;" ::: "memory");
             for (uint32_t i = 0; i < head; ++i) {
@@ -514,7 +516,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
         uint32_t s = 0, ph = 1;
         for (uint32_t i = head; i < k1 - k0; ++i) {
-            if (!(ok = wait(empty(s), ph ^ 1, abortp, 11))) break;
+            if (!wait(empty(s), ph ^ 1, abortp, 11)) break;
             if (elected()) {
                 weights(k0 + i, s);
                 tokens(k0 + i, s);
@@ -522,7 +524,6 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             __syncwarp();
             if (++s == p.stages) { s = 0; ph ^= 1; }
         }
-        if (!ok) leave_copies_behind();
     } else if (warp == 1) {
         if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");   // the launch in front may take longer than a wait on a barrier may
         bool ok = true, issued = false;
@@ -627,6 +628,8 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             gather(integral_constant<int, 1>{}, integral_constant<int, 8>{});
         }
     }
+    if (abort_flag && warp == 0) leave_copies_behind();   // whichever wait ran out: copies may be under way although every load was issued
+    __syncwarp();
     if (p.splits > 1) cluster_barrier();   // the others have read this CTA's partial sums
     if (p.early == 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // this launch does not end before the one in front
 }
