@@ -52,6 +52,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         }
     }
 }
+// A CTA in which a wait ran out lets its copies land before it gives its shared memory back. Called where it
+// does not matter which warp gave up (behind a barrier of the CTA): the one that consumes may, when the producer has long
+// issued its last copy.
+__device__ __forceinline__ void leave_copies_behind() {
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
+}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y, int z) {
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"

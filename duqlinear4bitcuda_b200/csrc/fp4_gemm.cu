@@ -151,12 +151,6 @@ __device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap *map, ui
     else
         tma_load_3d(dst, map, bar, x, y, z);
 }
-// A CTA in which a wait ran out lets its copies land before it gives its shared memory back. Called behind a barrier of the CTA, so
-// that it does not matter which warp gave up: the one that consumes may, when the producer has long issued its last copy.
-__device__ __forceinline__ void leave_copies_behind() {
-    const uint64_t t0 = globaltimer();
-    while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
-}
 
 // ---- many tokens: CTA pairs -------------------------------------------------------------------------------------
 struct PairArgs {

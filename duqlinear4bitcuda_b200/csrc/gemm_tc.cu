@@ -162,10 +162,6 @@ __global__ void __launch_bounds__(threads_for(UW), 1) gemm_tc_kernel(const __gri
                     }
                 }
             }
-            if (!ok) {  // give copies already in flight time to land before the CTA retires
-                uint64_t t0 = globaltimer();
-                while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
-            }
         }
     } else if (MODE == MODE_A8B4 && warp == kLastWarp) {
         // ---------------- second TMA producer: pre-unpacked A straight into the MMA ring ----------------
@@ -182,10 +178,6 @@ __global__ void __launch_bounds__(threads_for(UW), 1) gemm_tc_kernel(const __gri
                     mbar_expect_tx(up_full(u), BM * BK);
                     tma_load_3d(up0 + u * C::kUnpackedStage, &tmA, up_full(u), ks * BK, tm * BM, b);
                 }
-            }
-            if (!ok) {
-                uint64_t t0 = globaltimer();
-                while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
             }
         }
     } else if (warp == 1) {
@@ -285,6 +277,7 @@ __global__ void __launch_bounds__(threads_for(UW), 1) gemm_tc_kernel(const __gri
 
     tc_fence_before();
     __syncthreads();
+    if (abort_flag && warp == 0) leave_copies_behind();
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();

@@ -390,10 +390,6 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     tma_load_3d(dst, &tmB, pk_full(s), ks * (BKE / 2), wrow, b);
                 }
             }
-            if (!ok) {
-                uint64_t t0 = globaltimer();
-                while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
-            }
         }
     } else if (!APK && warp == kLastWarp) {
         // ---------------- TMA producer: this CTA's 128 rows of A, credited to the leader ----------------
@@ -410,10 +406,6 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
                     if (rank == 0) mbar_expect_tx(up_full(u), 2 * BMH * BKE + (WI8 ? 2 * bnh * BKE : 0));   // both CTAs' A tiles (and int8 W halves)
                     tma_load_3d_pair(up0 + u * kUnpackedStage, &tmA, mapa(up_full(u), 0), ks * BKE, tm * 256 + rank * BMH, b);
                 }
-            }
-            if (!ok) {
-                uint64_t t0 = globaltimer();
-                while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
             }
         }
     } else if (warp == 1) {
@@ -599,6 +591,8 @@ gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
 
     tc_fence_before();
     __syncthreads();
+    if (abort_flag && warp == 0) leave_copies_behind();
+    __syncwarp();
     cluster_sync_all();   // the partner has finished with this CTA's shared memory and its own TMEM
     if (warp == 1) {
         __syncwarp();

@@ -353,10 +353,7 @@ gemv_w4a4_tma_kernel(const __grid_constant__ CUtensorMap tmW, const uint8_t *__r
                         tma_load_3d(dst + j * (128u * S::kRows), &tmW, full(s), (int)(k0 + j * 128u), (int)row0, (int)b);
                 }
             }
-            if (!ok) {  // let copies already issued land before the CTA retires
-                uint64_t t0 = globaltimer();
-                while (globaltimer() - t0 < 200000ull) __nanosleep(1000);
-            }
+            if (!ok || *abortp) leave_copies_behind();   // copies already issued land before the CTA retires
         }
     } else {
         // ---------------- consumers ----------------
@@ -462,6 +459,7 @@ gemv_w4a4_tma_kernel(const __grid_constant__ CUtensorMap tmW, const uint8_t *__r
                 }
             }
         }
+        if (!ok) leave_copies_behind();   // the producer may have issued its last copy long ago
     }
 }
 
