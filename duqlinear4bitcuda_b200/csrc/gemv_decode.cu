@@ -51,12 +51,10 @@ __device__ __forceinline__ void fq_quantize(const FusedQ &fq, uint32_t M, uint32
         default: quantize_tokens_to_smem<QASYM_DUAL>(fq.x, M, K, fq.clip, raw, codes, stride, sc, kGemvWarps * 32); break;
     }
 }
-// 16 bytes of token codes: global memory (read-only path) or the CTA's shared memory
-template <bool FQ>
-__device__ __forceinline__ uint4 ld_codes(const uint4 *p) {
-    if (FQ) return *p;
-    return __ldg(p);
-}
+// 16 bytes of token codes: global memory or the CTA's shared memory. Not through the read-only path, and the kernels' A is not
+// __restrict__: with the promise on weights the launch in front may still write the codes while this grid is resident, and
+// read-only loads need not stay behind the wait for it.
+__device__ __forceinline__ uint4 ld_codes(const uint4 *p) { return *p; }
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
@@ -106,7 +104,7 @@ __device__ __forceinline__ uint4 ldg_stream(const uint4 *p) {
 // R  = 16-row weight groups per CTA (1 or 2); TH = token halves (1: M <= 8, 2: M <= 16); FQ: A is unused and the
 // tokens come as fp16 through `fq` (see FusedQ).
 template <int R, int TH, bool FQ>
-__global__ void __launch_bounds__(kGemvWarps * 32) gemv_w4a4_kernel(const uint8_t *__restrict__ A,
+__global__ void __launch_bounds__(kGemvWarps * 32) gemv_w4a4_kernel(const uint8_t *A,
                                                                     const uint8_t *__restrict__ W, uint32_t M, uint32_t N,
                                                                     uint32_t K, EpiParams p, __half *__restrict__ out,
                                                                     int32_t *__restrict__ acc_out, FusedQ fq) {
@@ -205,7 +203,7 @@ __global__ void __launch_bounds__(kGemvWarps * 32) gemv_w4a4_kernel(const uint8_
             uint32_t ch = (s0 + u) * 4 + t;
             bool ok = ch < nchunk;
 #pragma unroll
-            for (int h = 0; h < TH; ++h) av[u][h] = (ok && aok[h]) ? ld_codes<FQ>(ap[h] + ch) : make_uint4(0, 0, 0, 0);
+            for (int h = 0; h < TH; ++h) av[u][h] = (ok && aok[h]) ? ld_codes(ap[h] + ch) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -295,7 +293,7 @@ struct GemvSmem {
 
 template <int R, int TH, bool FQ>
 __global__ void __launch_bounds__((kGemvWarps + 1) * 32, 1)
-gemv_w4a4_tma_kernel(const __grid_constant__ CUtensorMap tmW, const uint8_t *__restrict__ A, uint32_t M, uint32_t N,
+gemv_w4a4_tma_kernel(const __grid_constant__ CUtensorMap tmW, const uint8_t *A, uint32_t M, uint32_t N,
                      uint32_t K, uint32_t batch, EpiParams p0, __half *__restrict__ out0, int32_t *__restrict__ acc0, FusedQ fq) {
     using namespace ptx;
     using S = GemvSmem<R>;
@@ -386,8 +384,8 @@ gemv_w4a4_tma_kernel(const __grid_constant__ CUtensorMap tmW, const uint8_t *__r
                     const uint32_t m = g + 8 * h;
                     const bool lok = kin && m < M;
                     const uint4 *ap = reinterpret_cast<const uint4 *>(Ab + (size_t)(lok ? m : 0) * a_stride + (lok ? kbyte : 0));
-                    tk[h][0] = lok ? ld_codes<FQ>(ap) : make_uint4(0, 0, 0, 0);
-                    tk[h][1] = lok ? ld_codes<FQ>(ap + 1) : make_uint4(0, 0, 0, 0);
+                    tk[h][0] = lok ? ld_codes(ap) : make_uint4(0, 0, 0, 0);
+                    tk[h][1] = lok ? ld_codes(ap + 1) : make_uint4(0, 0, 0, 0);
                 }
                 if (ok) ok = mbar_wait(full(s), ph, abortp, &g_gemv_status, 2);
                 if (ok && ks * kStageKBytes + warp * 128u < kb) {
@@ -570,7 +568,7 @@ struct GemvBuf {
 
 template <int TH, int U, bool FQ>
 __global__ void __launch_bounds__(kGemvWarps * 32, 2)
-gemv_w4a4_persist_kernel(const uint8_t *__restrict__ A, const uint8_t *__restrict__ W, uint32_t M, uint32_t N, uint32_t K,
+gemv_w4a4_persist_kernel(const uint8_t *A, const uint8_t *__restrict__ W, uint32_t M, uint32_t N, uint32_t K,
                          uint32_t batch, EpiParams p0, __half *__restrict__ out0, int32_t *__restrict__ acc0, FusedQ fq) {
     extern __shared__ __align__(16) uint8_t fq_smem[];
     TokenQuantScratch &qsc = *reinterpret_cast<TokenQuantScratch *>(fq_smem);
@@ -615,7 +613,7 @@ gemv_w4a4_persist_kernel(const uint8_t *__restrict__ A, const uint8_t *__restric
             for (int h = 0; h < TH; ++h) {
                 const uint32_t m = g + 8 * h;
                 const bool ok = ch < nchunk && m < M;
-                buf.a[u][h] = ok ? ld_codes<FQ>(reinterpret_cast<const uint4 *>(Ab + (size_t)m * a_stride) + ch) : make_uint4(0, 0, 0, 0);
+                buf.a[u][h] = ok ? ld_codes(reinterpret_cast<const uint4 *>(Ab + (size_t)m * a_stride) + ch) : make_uint4(0, 0, 0, 0);
             }
         }
     };

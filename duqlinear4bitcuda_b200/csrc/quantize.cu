@@ -73,7 +73,7 @@ __device__ __forceinline__ uint4 silu_mul8(const uint4 &g, const uint4 &u) {
 // silu(x[row, 0:cols]) * x[row, up_off : up_off+cols] of a [rows, in_stride] gate/up tensor, i.e. the
 // activation of a SiLU-gated MLP is formed, measured and quantized without ever being stored in fp16.
 template <int MODE, int VPT, bool SILU = false, int NT = 256>
-__global__ void __launch_bounds__(NT) quant_fused_vec_kernel(const __half *__restrict__ x, uint32_t rows, uint32_t cols,
+__global__ void __launch_bounds__(NT) quant_fused_vec_kernel(const __half *x, uint32_t rows, uint32_t cols,
                                                               float clip, uint8_t *__restrict__ q, __half *s1o,
                                                               __half *z1o, __half *s2o, __half *z2o, bool out8,
                                                               uint32_t in_stride = 0, uint32_t up_off = 0) {
@@ -82,6 +82,9 @@ __global__ void __launch_bounds__(NT) quant_fused_vec_kernel(const __half *__res
     // Programmatic dependent launch (both instructions do nothing unless the launch carries the attribute): the
     // kernel that follows on the stream -- the small-M linear kernel, which streams weights before it needs these
     // codes -- may start right away; this kernel itself touches memory only after the stream's earlier work is done.
+    // The tokens may be written while this grid is resident already, so they are not read through the read-only path (and
+    // x is not __restrict__, which would let the compiler choose it): such loads need not stay behind the wait. The SiLU
+    // form is never launched with the attribute and keeps them (4096 x 11008: 80.0 us, 82.0 without).
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     for (uint32_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -93,8 +96,8 @@ __global__ void __launch_bounds__(NT) quant_fused_vec_kernel(const __half *__res
         for (int i = 0; i < VPT; ++i) {
             uint32_t v = threadIdx.x + i * NT;
             if (v < nvec) {
-                d[i] = __ldg(xr + v);
-                if (SILU) d[i] = silu_mul8(d[i], __ldg(xr + (up_off >> 3) + v));
+                if (SILU) d[i] = silu_mul8(__ldg(xr + v), __ldg(xr + (up_off >> 3) + v));
+                else d[i] = xr[v];
             }
         }
         // Row statistics on the raw bit patterns: for symmetric schemes the integer maximum of
