@@ -110,6 +110,15 @@ class LinearFP4(torch.nn.Module):
         else:
             self.bias = None
 
+    def _apply(self, fn, recurse=True):
+        # .half(), .to(dtype) and the like convert every floating-point buffer of a model; the row scales are part of the
+        # format, 32 bits whatever the layer's type, and only follow the device
+        rows = self.weight_row_scales
+        super()._apply(fn, recurse)
+        if rows is not None and self.weight_row_scales.dtype != torch.float32:
+            self.weight_row_scales = rows.to(self.weight_row_scales.device)
+        return self
+
     def forward(self, x):
         w = (self.weight, self.weight_scales, self.weight_row_scales)
         if isinstance(x, PackedFP4Tensor):
