@@ -91,7 +91,8 @@ class LinearFP4(torch.nn.Module):
     """Linear layer on microscaled 4-bit weights and activations. Buffers: weight uint8 [out, in/2], weight_scales uint8
     (block scales in the tensor cores' tile order; qz.fp4_tile_scales makes it from [out, in/block]), weight_row_scales
     float [out] (the nvfp4 format's second scale; a checkpoint's one float per tensor is that float in every row), bias.
-    forward takes 16-bit activations (quantized on the way, the result has their type) or a PackedFP4Tensor."""
+    forward takes 16-bit activations (quantized on the way, the result has their type) or a PackedFP4Tensor; a bias of another
+    type than theirs is rounded to it in every call."""
 
     def __init__(self, in_features, out_features, bias=False, format="nvfp4", dtype=torch.float16):
         super().__init__()
@@ -119,22 +120,27 @@ class LinearFP4(torch.nn.Module):
             self.weight_row_scales = rows.to(self.weight_row_scales.device)
         return self
 
+    def _bias_as(self, dtype):
+        return self.bias if self.bias is None or self.bias.dtype == dtype else self.bias.to(dtype)
+
     def forward(self, x):
         w = (self.weight, self.weight_scales, self.weight_row_scales)
         if isinstance(x, PackedFP4Tensor):
             if x.format != self.format:
                 raise ValueError(f"activations are {x.format}, the weights {self.format}")
             codes, lead = _as_rows(x.codes)
-            y = ops.linear_fp4(self.format, codes, x.block_scales, x.row_scales, *w, self.bias, x.dtype)
+            y = ops.linear_fp4(self.format, codes, x.block_scales, x.row_scales, *w, self._bias_as(x.dtype), x.dtype)
         else:
             x2, lead = _as_rows(x)
-            y = ops.linear_fp4_from_16bit(self.format, x2, *w, self.bias)
+            y = ops.linear_fp4_from_16bit(self.format, x2, *w, self._bias_as(x.dtype))
         return y.view(*lead, self.out_features)
 
     @classmethod
-    def from_linear(cls, module: torch.nn.Linear, format="nvfp4", dtype=torch.float16):
+    def from_linear(cls, module: torch.nn.Linear, format="nvfp4", dtype=None):
         """Quantizes the weights of a Linear on the GPU; the buffers stay there. dtype: of the bias, that is of the
-        activations the layer will see."""
+        activations the layer will see; the module's own where that has 16 bits, else fp16."""
+        if dtype is None:
+            dtype = module.weight.dtype if module.weight.dtype in (torch.float16, torch.bfloat16) else torch.float16
         new = cls(module.in_features, module.out_features, module.bias is not None, format, dtype)
         w = module.weight.data
         if w.dtype not in (torch.float16, torch.bfloat16):

@@ -1,0 +1,46 @@
+"""Modules of the fp4 operators as a model uses them: types of a layer and of its activations."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+H, B = torch.float16, torch.bfloat16
+
+
+def layer(dtype):
+    torch.manual_seed(3)
+    return torch.nn.Linear(128, 72, bias=True).to(dtype).cuda()
+
+
+def product(q, x, bias):
+    """The operator itself on the layer's weights, with a bias of the activations' type."""
+    import duqlinear4bitcuda_b200._CUDA as o
+    return o.linear_fp4_from_16bit(q.format, x, q.weight, q.weight_scales, q.weight_row_scales, bias)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("own", [H, B])
+def test_a_layer_takes_its_own_activations(fmt, own):
+    """from_linear keeps the type of a 16-bit layer, so that what the layer took the new one takes."""
+    import duqlinear4bitcuda_b200.nn as nn
+    lin = layer(own)
+    q = nn.LinearFP4.from_linear(lin, fmt)
+    assert q.bias.dtype == own and torch.equal(q.bias, lin.bias)
+    x = torch.randn(5, 128, device="cuda").to(own)
+    y = q(x)
+    assert y.dtype == own and torch.equal(y, product(q, x, lin.bias.detach()))
+    assert torch.equal(q(nn.QuantizerFP4(fmt)(x)), y)
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("own,given,acts", [(torch.float32, None, H), (torch.float32, B, B), (B, H, H), (H, B, B),
+                                            (B, None, H), (H, None, B), (torch.float32, None, B)])
+def test_a_bias_of_another_type_is_rounded_to_the_activations(fmt, own, given, acts):
+    import duqlinear4bitcuda_b200.nn as nn
+    lin = layer(own)
+    q = nn.LinearFP4.from_linear(lin, fmt) if given is None else nn.LinearFP4.from_linear(lin, fmt, given)
+    kept = given or (own if own in (H, B) else H)
+    assert q.bias.dtype == kept
+    x = torch.randn(3, 128, device="cuda").to(acts)
+    want = product(q, x, lin.bias.detach().to(kept).to(acts))
+    assert torch.equal(q(x), want) and torch.equal(q(nn.QuantizerFP4(fmt)(x)), want)
+    assert torch.equal(q.float()(x), want)      # a bias that a conversion of the model left in 32 bits
