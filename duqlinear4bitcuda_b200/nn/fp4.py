@@ -54,13 +54,13 @@ class NormResidualQuantizer(torch.nn.Module):
 
     norm(t) = t / sqrt(mean(t^2) + eps) over the last dimension. gate: None, [dim], or like x. format: "mxfp4" / "nvfp4" (a
     PackedFP4Tensor for LinearFP4), "sym" / "asym" (a PackedQuantizedTensor for the integer layers, fp16), "none" (the norm
-    itself). dim % 32 == 0."""
+    itself). input_clip_ratio: as SymQuantizer's, for "sym" only. dim % 32 == 0."""
 
-    def __init__(self, dim, format="nvfp4", eps=1e-6, post_norm=False, residual_scale=1.0, dtype=torch.float16):
+    def __init__(self, dim, format="nvfp4", eps=1e-6, post_norm=False, residual_scale=1.0, dtype=torch.float16, input_clip_ratio=1.0):
         super().__init__()
         if format not in ("none", "sym", "asym"):
             _check_format(format)
-        self.format, self.eps, self.residual_scale = format, eps, residual_scale
+        self.format, self.eps, self.residual_scale, self.input_clip_ratio = format, eps, residual_scale, input_clip_ratio
         self.register_buffer("weight", torch.ones(dim, dtype=dtype))
         if post_norm:
             self.register_buffer("post_weight", torch.ones(dim, dtype=dtype))
@@ -75,7 +75,8 @@ class NormResidualQuantizer(torch.nn.Module):
             post = self.post_weight
             if gate is not None and gate.dim() > 1:
                 gate = _as_rows(gate)[0]
-        stream, *q = ops.norm_residual_quantize(self.format, x2, self.weight, self.eps, residual, post, gate, self.residual_scale)
+        stream, *q = ops.norm_residual_quantize(self.format, x2, self.weight, self.eps, residual, post, gate, self.residual_scale,
+                                               self.input_clip_ratio)
         if self.format == "none":
             out = q[0].view(x.shape)
         elif self.format == "sym":

@@ -28,3 +28,28 @@ def test_row_scales_follow_the_device():
     assert m.weight_row_scales.device.type == "meta" and m.weight_row_scales.dtype == torch.float32
     m = m.half().to_empty(device="cpu")
     assert m.weight_row_scales.device.type == "cpu" and m.weight_row_scales.dtype == torch.float32
+
+
+class Recorder:
+    """Stands in for the operator module: notes the call and gives back results of the right shapes."""
+
+    def norm_residual_quantize(self, *args):
+        self.args = args
+        x, residual = args[1], args[4]
+        rows, cols = x.shape
+        return residual, torch.zeros(rows, cols // 2, dtype=torch.uint8), torch.zeros(rows, dtype=H), torch.zeros(rows, dtype=H)
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    r = Recorder()
+    monkeypatch.setattr(nn.fp4, "ops", r)
+    return r
+
+
+@pytest.mark.parametrize("given,want", [({}, 1.0), ({"input_clip_ratio": 0.75}, 0.75)])
+def test_clip_ratio_reaches_the_quantizer(recorder, given, want):
+    """As SymQuantizer's."""
+    q = nn.NormResidualQuantizer(64, "sym", **given)
+    q(torch.zeros(3, 64, dtype=H))
+    assert recorder.args[8] == want and q.input_clip_ratio == want

@@ -44,3 +44,13 @@ def test_a_bias_of_another_type_is_rounded_to_the_activations(fmt, own, given, a
     want = product(q, x, lin.bias.detach().to(kept).to(acts))
     assert torch.equal(q(x), want) and torch.equal(q(nn.QuantizerFP4(fmt)(x)), want)
     assert torch.equal(q.float()(x), want)      # a bias that a conversion of the model left in 32 bits
+
+
+@pytest.mark.parametrize("ratio", [1.0, 0.8])
+def test_joint_with_a_clip_ratio_equals_the_quantizer(ratio):
+    import duqlinear4bitcuda_b200.nn as nn
+    x, r = torch.randn(7, 96, device="cuda").half(), torch.randn(7, 96, device="cuda").half()
+    h, _ = nn.NormResidualQuantizer(96, "none").cuda()(x, r)
+    got, _ = nn.NormResidualQuantizer(96, "sym", input_clip_ratio=ratio).cuda()(x, r)
+    want = nn.SymQuantizer(ratio)(h)
+    assert torch.equal(got.quantized_x, want.quantized_x) and torch.equal(got.scales_x, want.scales_x)
