@@ -44,6 +44,18 @@ class SiluMulQuantizerFP4(torch.nn.Module):
         return _packed(self.format, ops.fp4_silu_mul_quantize(self.format, x2), lead, gate_up.dtype)
 
 
+def _rows_of(name, t, x, rows, broadcast):
+    """t as the rows [rows, C] of x: of x's shape but for leading ones, flattened already, or (a gate) whatever broadcasts to
+    x's shape. As many rows in another arrangement are refused: they would meet the wrong tokens."""
+    while t.dim() > x.dim() and t.shape[0] == 1:
+        t = t[0]
+    if t.shape == x.shape or t.shape == (rows, x.shape[-1]):
+        return _as_rows(t)[0]
+    if t.dim() > x.dim() or any(a not in (1, b) for a, b in zip(t.shape[::-1], x.shape[::-1])) or not (broadcast or t.numel() == x.numel()):
+        raise ValueError(f"{name} of shape {tuple(t.shape)} does not go with x of shape {tuple(x.shape)}")
+    return _as_rows(t.expand(x.shape))[0]
+
+
 class NormResidualQuantizer(torch.nn.Module):
     """The joint between two blocks of a transformer in one kernel: the norm after a block (post_norm=True), its gate and
     residual scale, the residual sum, the norm before the next block, and the quantizer in front of its first layer.
@@ -52,9 +64,9 @@ class NormResidualQuantizer(torch.nn.Module):
         forward(x, residual, gate)  -> (quantized norm(r) * weight, r),
                                        r = residual + residual_scale * gate * [norm(x) * post_weight]
 
-    norm(t) = t / sqrt(mean(t^2) + eps) over the last dimension. gate: None, [dim], or like x. format: "mxfp4" / "nvfp4" (a
-    PackedFP4Tensor for LinearFP4), "sym" / "asym" (a PackedQuantizedTensor for the integer layers, fp16), "none" (the norm
-    itself). input_clip_ratio: as SymQuantizer's, for "sym" only. dim % 32 == 0."""
+    norm(t) = t / sqrt(mean(t^2) + eps) over the last dimension. residual: like x. gate: None, [dim], or what broadcasts to x
+    (one per sequence, [B, 1, dim], is copied to one per token). format: "mxfp4" / "nvfp4" (a PackedFP4Tensor for
+    LinearFP4), "sym" / "asym" (a PackedQuantizedTensor for the integer layers, fp16), "none" (the norm itself). input_clip_ratio: as SymQuantizer's, for "sym" only. dim % 32 == 0."""
 
     def __init__(self, dim, format="nvfp4", eps=1e-6, post_norm=False, residual_scale=1.0, dtype=torch.float16, input_clip_ratio=1.0):
         super().__init__()
@@ -71,10 +83,12 @@ class NormResidualQuantizer(torch.nn.Module):
         x2, lead = _as_rows(x)
         post = None
         if residual is not None:
-            residual = _as_rows(residual)[0]
+            residual = _rows_of("residual", residual, x, x2.shape[0], False)
             post = self.post_weight
-            if gate is not None and gate.dim() > 1:
-                gate = _as_rows(gate)[0]
+            if gate is not None and gate.dim() > 1 and gate.numel() == gate.shape[-1]:
+                gate = gate.reshape(-1)   # one for all tokens
+            if gate is not None and gate.shape != x.shape[-1:]:
+                gate = _rows_of("gate", gate, x, x2.shape[0], True)
         stream, *q = ops.norm_residual_quantize(self.format, x2, self.weight, self.eps, residual, post, gate, self.residual_scale,
                                                self.input_clip_ratio)
         if self.format == "none":

@@ -53,3 +53,47 @@ def test_clip_ratio_reaches_the_quantizer(recorder, given, want):
     q = nn.NormResidualQuantizer(64, "sym", **given)
     q(torch.zeros(3, 64, dtype=H))
     assert recorder.args[8] == want and q.input_clip_ratio == want
+
+
+def joint(recorder, x, residual, gate=None):
+    out, stream = nn.NormResidualQuantizer(64, "sym")(x, residual, gate)
+    assert stream.shape == x.shape
+    return recorder.args[4], recorder.args[6]
+
+
+X = torch.arange(2 * 3 * 64).reshape(2, 3, 64).to(H)
+
+
+@pytest.mark.parametrize("shape", [(3, 2, 64), (6, 1, 64), (2, 3, 32), (1, 3, 64), (64,), (5, 64)])
+def test_residual_of_another_shape_is_refused(recorder, shape):
+    """As many rows in another arrangement would pair tokens with tokens of other sequences."""
+    with pytest.raises(ValueError, match="residual"):
+        joint(recorder, X, torch.zeros(shape, dtype=H))
+
+
+@pytest.mark.parametrize("shape", [(3, 2, 64), (6, 1, 64), (32,), (2, 64), (3, 1, 64), (2, 3, 1, 64), (5, 64)])
+def test_gate_of_another_shape_is_refused(recorder, shape):
+    with pytest.raises(ValueError, match="gate"):
+        joint(recorder, X, X, torch.zeros(shape, dtype=H))
+
+
+@pytest.mark.parametrize("x,shape", [(X, (2, 3, 64)), (X, (6, 64)), (X[:1], (3, 64)), (X[:1], (1, 3, 64)), (X[0], (1, 3, 64)), (X[0, 0], (64,)), (X[0, 0], (1, 1, 64))])
+def test_residual_shapes(recorder, x, shape):
+    r = torch.randn(shape).to(H)
+    assert torch.equal(joint(recorder, x, r)[0], r.reshape(-1, 64))
+
+
+@pytest.mark.parametrize("shape", [(64,), (1, 64), (1, 1, 64)])
+def test_one_gate_for_all_tokens_is_handed_on_as_it_is(recorder, shape):
+    g = torch.randn(shape).to(H)
+    got = joint(recorder, X, X, g)[1]
+    assert got.shape == (64,) and torch.equal(got, g.reshape(64)) and got.data_ptr() == g.data_ptr()
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 64), (6, 64), (2, 1, 64), (1, 3, 64), (3, 64)])
+def test_gates_of_tokens_sequences_and_positions(recorder, shape):
+    """Whatever broadcasts to x: a gate per token, per sequence, per position."""
+    g = torch.randn(shape).to(H)
+    got = joint(recorder, X, X, g)[1]
+    want = g if shape == (6, 64) else (torch.ones(2, 3, 64, dtype=H) * g).reshape(6, 64)
+    assert got.is_contiguous() and torch.equal(got, want)

@@ -54,3 +54,15 @@ def test_joint_with_a_clip_ratio_equals_the_quantizer(ratio):
     got, _ = nn.NormResidualQuantizer(96, "sym", input_clip_ratio=ratio).cuda()(x, r)
     want = nn.SymQuantizer(ratio)(h)
     assert torch.equal(got.quantized_x, want.quantized_x) and torch.equal(got.scales_x, want.scales_x)
+
+
+@pytest.mark.parametrize("shape", [(128,), (1, 1, 128), (4, 1, 128), (1, 5, 128), (4, 5, 128), (20, 128)])
+def test_joint_with_gates_that_broadcast(shape):
+    """A gate per channel, sequence, position and token equals the same gate written out for every token."""
+    import duqlinear4bitcuda_b200.nn as nn
+    x, r, g = torch.randn(4, 5, 128, device="cuda").to(B), torch.randn(4, 5, 128, device="cuda").to(B), torch.randn(shape, device="cuda").to(B)
+    joint = nn.NormResidualQuantizer(128, "nvfp4", post_norm=True, dtype=B).cuda()
+    q, stream = joint(x, r, g)
+    full = (g.view(4, 5, 128) if shape == (20, 128) else g.expand(4, 5, 128)).contiguous()
+    want, wstream = joint(x, r, full)
+    assert torch.equal(q.codes, want.codes) and torch.equal(stream, wstream) and torch.equal(q.dequantize(), want.dequantize())
