@@ -765,33 +765,39 @@ static uint64_t swap_price(uint32_t M, uint64_t tiles, uint64_t ktiles, uint64_t
     const uint64_t splits = swap_splits(M, tiles, ktiles, sms);
     return (tiles * splits + sms - 1) / sms * ((ktiles + splits - 1) / splits) * 50 + (splits > 1 ? 1120 : 810);
 }
-template <int FMT, class T>
-static int gemm(const GemmArgs &a, cudaStream_t st, uint32_t early) {
-    if (a.M <= 128) return launch_swap<FMT, T>(a, st, early);
-    const uint64_t sms = sm_count_current_device(), ktiles = cdiv(a.K, (uint32_t)kBK), tiles_m = cdiv(a.M, 256), tiles_n = cdiv(a.N, 256);
-    const uint64_t blocks_m = cdiv(a.M, 128), pairs = pair_price(tiles_m * tiles_n, ktiles, sms);
+// The columns of the result that the pair kernel computes: none, all, or whole rounds of its tiles, the columns that are left
+// being the other kernel's (they begin at a multiple of 256, so at a whole tile of the weights' block scales).
+static uint32_t pair_columns(uint32_t M, uint32_t N, uint32_t K, uint64_t sms) {
+    if (M <= 128) return 0;
+    const uint64_t ktiles = cdiv(K, (uint32_t)kBK), tiles_m = cdiv(M, 256), tiles_n = cdiv(N, 256);
+    const uint64_t blocks_m = cdiv(M, 128), pairs = pair_price(tiles_m * tiles_n, ktiles, sms);
     const bool swap_fits = blocks_m <= 65535;   // the grid's second dimension
-    const uint64_t swap = swap_fits ? swap_price(a.M, blocks_m * cdiv(a.N, 128), ktiles, sms) : ~0ull, one = swap < pairs ? swap : pairs;
+    const uint64_t swap = swap_fits ? swap_price(M, blocks_m * cdiv(N, 128), ktiles, sms) : ~0ull, one = swap < pairs ? swap : pairs;
     // A last round that few tiles are left for: whole rounds by the pair kernel, the columns that are left by the other one,
     // launched behind it (512 x 28672 x 8192, 3 rounds and 2 tiles of 256 x 256).
     const uint64_t rest = tiles_m * tiles_n % (sms / 2), strip = rest ? (rest + tiles_m - 1) / tiles_m : 0;
     if (swap_fits && strip && strip < tiles_n) {
         const uint32_t n0 = (uint32_t)(tiles_n - strip) * 256;
-        const uint64_t both = pair_price(tiles_m * (tiles_n - strip), ktiles, sms) + swap_price(a.M, blocks_m * cdiv(a.N - n0, 128), ktiles, sms) + 160;
-        if (both < one) {
-            GemmArgs main = a, left = a;
-            main.N = n0;
-            left.N = a.N - n0;
-            left.w += (size_t)n0 * (a.K / 2);
-            left.w_scales += (size_t)(n0 / 128) * scale_tiles(FMT, a.K) * kTileBytes;
-            if (a.w_rows) left.w_rows += n0;
-            if (a.bias) left.bias = reinterpret_cast<const uint16_t *>(a.bias) + n0;
-            left.out = reinterpret_cast<uint16_t *>(a.out) + n0;
-            const int rc = launch_pair<FMT, T>(main, st);
-            return rc ? rc : launch_swap<FMT, T>(left, st, 2);
-        }
+        const uint64_t both = pair_price(tiles_m * (tiles_n - strip), ktiles, sms) + swap_price(M, blocks_m * cdiv(N - n0, 128), ktiles, sms) + 160;
+        if (both < one) return n0;
     }
-    return swap < pairs ? launch_swap<FMT, T>(a, st, early) : launch_pair<FMT, T>(a, st);
+    return swap < pairs ? 0 : N;
+}
+template <int FMT, class T>
+static int gemm(const GemmArgs &a, cudaStream_t st, uint32_t early) {
+    const uint32_t n0 = pair_columns(a.M, a.N, a.K, (uint64_t)sm_count_current_device());
+    if (n0 == 0) return launch_swap<FMT, T>(a, st, early);
+    if (n0 == a.N) return launch_pair<FMT, T>(a, st);
+    GemmArgs main = a, left = a;
+    main.N = n0;
+    left.N = a.N - n0;
+    left.w += (size_t)n0 * (a.K / 2);
+    left.w_scales += (size_t)(n0 / 128) * scale_tiles(FMT, a.K) * kTileBytes;
+    if (a.w_rows) left.w_rows += n0;
+    if (a.bias) left.bias = reinterpret_cast<const uint16_t *>(a.bias) + n0;
+    left.out = reinterpret_cast<uint16_t *>(a.out) + n0;
+    const int rc = launch_pair<FMT, T>(main, st);
+    return rc ? rc : launch_swap<FMT, T>(left, st, 2);
 }
 
 static int check_gemm(int format, int dtype, uint32_t M, uint32_t N, uint32_t K, uint64_t ldo) {
@@ -844,6 +850,10 @@ int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales,
         return DUQ4_ERR_ALIGN;
     const GemmArgs a{M, N, K, A, A_block_scales, W, W_block_scales, A_row_scales, W_row_scales, bias, out, ldo};
     return run(format, dtype, a, (cudaStream_t)stream, g_static_weights.load(std::memory_order_relaxed) ? 1 : 3);
+}
+
+uint32_t duq4_linear_fp4_pair_columns(uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {
+    return sms < 2 || M == 0 || N == 0 || K == 0 || (M | N | K) > 0x7FFFFFFFu ? 0 : pair_columns(M, N, K, sms);
 }
 
 size_t duq4_linear_fp4_workspace_bytes(int format, uint32_t M, uint32_t K) {

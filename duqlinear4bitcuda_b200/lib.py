@@ -123,6 +123,7 @@ SIGNATURES = {
     "duq4_fp4_dequantize": [_i, _i, _vp, _vp, _vp, _u32, _u32, _vp, _vp],
     "duq4_norm_residual_quantize": [_i, ctypes.POINTER(NormResidual), _u32, _u32, _vp, _vp, _vp, _vp],
     "duq4_linear_fp4": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _i, _vp, _u64, _vp],
+    "duq4_linear_fp4_pair_columns": [_u32, _u32, _u32, _u32],
     "duq4_linear_fp4_workspace_bytes": [_i, _u32, _u32],
     "duq4_linear_fp4_from_16bit": [_i, _i, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _u64, _vp, _sz, _vp],
     "duq4_peer_barrier": [ctypes.POINTER(ctypes.c_void_p), _u32, _u32, ctypes.c_uint64, ctypes.c_uint64, _vp],
@@ -131,7 +132,7 @@ SIGNATURES = {
 _RESTYPES = {"duq4_version": ctypes.c_char_p, "duq4_error_string": ctypes.c_char_p,
              "duq4_linear_from_fp16_workspace_bytes": ctypes.c_size_t, "duq4_gemm_split_scratch_bytes": ctypes.c_size_t,
              "duq4_linear_from_fp16_prelaid_workspace_bytes": ctypes.c_size_t,
-             "duq4_fp4_scale_bytes": ctypes.c_size_t, "duq4_linear_fp4_workspace_bytes": ctypes.c_size_t,
+             "duq4_linear_fp4_pair_columns": ctypes.c_uint32, "duq4_fp4_scale_bytes": ctypes.c_size_t, "duq4_linear_fp4_workspace_bytes": ctypes.c_size_t,
              "duq4_linear_host_staging_bytes": ctypes.c_size_t, "duq4_linear_pipeline_staging_bytes": ctypes.c_size_t}
 
 if not os.path.exists(LIB_PATH):

@@ -536,6 +536,9 @@ int duq4_norm_residual_quantize(int format, const duq4_norm_residual *n, uint32_
 int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales, const float *A_row_scales, const uint8_t *W,
                     const uint8_t *W_block_scales, const float *W_row_scales, uint32_t M, uint32_t N, uint32_t K, const void *bias, int dtype,
                     void *out, uint64_t ldo, void *stream);
+/* Which kernels such a product runs on a GPU of `sms` SMs: how many of its N columns the CTA-pair kernel computes. 0: none, all
+ * are the few-token kernel's; N: all; between: the rest is a second launch. Host arithmetic only; tests hold their sizes to it. */
+uint32_t duq4_linear_fp4_pair_columns(uint32_t M, uint32_t N, uint32_t K, uint32_t sms);
 /* The same from 16-bit activations x [M, K] (dense): quantized into `workspace` (device memory, 256-byte aligned,
  * duq4_linear_fp4_workspace_bytes bytes), then multiplied. Calls that share a workspace must not overlap on the GPU. */
 size_t duq4_linear_fp4_workspace_bytes(int format, uint32_t M, uint32_t K);
