@@ -44,13 +44,25 @@ struct GemmArgs {
 constexpr int kBK = 256;            // K per stage: 128 bytes of codes per row
 constexpr int kTileBytes = 512;     // scale tile: 128 rows x 4 blocks
 
-__device__ __forceinline__ void fp4_fail(volatile int *abort_flag, int code) {
-    *abort_flag = 1;
-    atomicCAS(&g_fp4_status, 0, code);
-}
 // Bounded wait on a barrier of this CTA (arrivals may come from the partner).
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int code) {
     return mbar_wait(bar, parity, abort_flag, &g_fp4_status, code);
+}
+
+// The wait itself, run out: one warp waits on a barrier that nothing arrives at. `gave_up`: 1 if the first wait reported so, 2 more
+// if the next one, with the CTA aborting, did not wait again.
+__global__ void fp4_wait_selftest_kernel(int *gave_up) {
+    __shared__ int abort_flag;
+    __shared__ __align__(8) uint64_t bar;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        mbar_init(smem_u32(&bar), 1);
+    }
+    __syncthreads();
+    const bool first = wait(smem_u32(&bar), 0, &abort_flag, 14);
+    const uint64_t t0 = globaltimer();
+    const bool second = wait(smem_u32(&bar), 0, &abort_flag, 15);
+    if (threadIdx.x == 0) *gave_up = (first ? 0 : 1) + (!second && globaltimer() - t0 < kPtxWaitLimitNs / 2 ? 2 : 0);
 }
 
 // Instruction descriptor of the block-scaled kinds: e2m1 x e2m1 -> f32, both operands K-major. (Bits 4-5 and 29-30 name the
@@ -850,6 +862,14 @@ int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales,
         return DUQ4_ERR_ALIGN;
     const GemmArgs a{M, N, K, A, A_block_scales, W, W_block_scales, A_row_scales, W_row_scales, bias, out, ldo};
     return run(format, dtype, a, (cudaStream_t)stream, g_static_weights.load(std::memory_order_relaxed) ? 1 : 3);
+}
+
+int duq4_fp4_wait_selftest(int32_t *result, void *stream) {
+    DUQ4_TRACE();
+    if (!result) return DUQ4_ERR_NULL;
+    if (!aligned(result, 4)) return DUQ4_ERR_ALIGN;
+    fp4_wait_selftest_kernel<<<1, 32, 0, (cudaStream_t)stream>>>(result);
+    return launch_status();
 }
 
 uint32_t duq4_linear_fp4_pair_columns(uint32_t M, uint32_t N, uint32_t K, uint32_t sms) {

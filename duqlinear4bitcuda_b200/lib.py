@@ -123,6 +123,7 @@ SIGNATURES = {
     "duq4_fp4_dequantize": [_i, _i, _vp, _vp, _vp, _u32, _u32, _vp, _vp],
     "duq4_norm_residual_quantize": [_i, ctypes.POINTER(NormResidual), _u32, _u32, _vp, _vp, _vp, _vp],
     "duq4_linear_fp4": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _i, _vp, _u64, _vp],
+    "duq4_fp4_wait_selftest": [_vp, _vp],
     "duq4_linear_fp4_pair_columns": [_u32, _u32, _u32, _u32],
     "duq4_linear_fp4_workspace_bytes": [_i, _u32, _u32],
     "duq4_linear_fp4_from_16bit": [_i, _i, _vp, _vp, _vp, _vp, _u32, _u32, _u32, _vp, _vp, _u64, _vp, _sz, _vp],

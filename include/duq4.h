@@ -536,6 +536,10 @@ int duq4_norm_residual_quantize(int format, const duq4_norm_residual *n, uint32_
 int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales, const float *A_row_scales, const uint8_t *W,
                     const uint8_t *W_block_scales, const float *W_row_scales, uint32_t M, uint32_t N, uint32_t K, const void *bias, int dtype,
                     void *out, uint64_t ldo, void *stream);
+/* Checks the product's failure detection on the current device: one warp runs a wait of the product's on a barrier that nothing
+ * arrives at. It gives up after its limit of one second, code 414 stands in the device status word, and *result (device memory)
+ * becomes 3 (1: the wait reported that it gave up, 2: the next one did not wait again). Nothing else is touched. */
+int duq4_fp4_wait_selftest(int32_t *result, void *stream);
 /* Which kernels such a product runs on a GPU of `sms` SMs: how many of its N columns the CTA-pair kernel computes. 0: none, all
  * are the few-token kernel's; N: all; between: the rest is a second launch. Host arithmetic only; tests hold their sizes to it. */
 uint32_t duq4_linear_fp4_pair_columns(uint32_t M, uint32_t N, uint32_t K, uint32_t sms);
@@ -558,8 +562,9 @@ int duq4_linear_fp4_from_16bit(int format, int dtype, const void *x, const uint8
 int duq4_peer_barrier(const void *const *flag_ptrs, uint32_t world, uint32_t rank, uint64_t epoch,
                       uint64_t timeout_ns, void *stream);
 
-/* Device-side status word of the most recent tensor-core GEMM on the current device:
- * 0 = no bounded wait expired. Reads back 4 bytes (synchronises the stream given). */
+/* Device-side status of the current device since the last such call: 0 = no bounded wait expired, else the code of one that did
+ * (1..9 tensor-core GEMM, 101.. small-M kernel, 201.. CTA-pair GEMM, 301 rank barrier, 401..413 fp4 product, 414 its self-test).
+ * Synchronises the stream given and starts over at 0. */
 int duq4_last_device_status(void *stream, int32_t *status_out /* host pointer */);
 
 #ifdef __cplusplus

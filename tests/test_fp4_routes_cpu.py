@@ -48,3 +48,7 @@ def test_bounds():
                 for sms in (2, 132, 148, 160):
                     n0 = pair_columns(m, n, k, sms)
                     assert n0 in (0, n) or (n0 % 256 == 0 and 0 < n0 < n)
+
+
+def test_selftest_refuses():
+    assert L.cdll.duq4_fp4_wait_selftest(None, None) == -1 and L.cdll.duq4_fp4_wait_selftest(0x1002, None) == -5
