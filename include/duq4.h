@@ -512,8 +512,9 @@ int duq4_fp4_dequantize(int format, int dtype, const uint8_t *codes, const uint8
  * x, residual, residual_out [rows, cols]; weights [cols]; gate [cols], or [rows, cols] with gate_per_row != 0; all of
  * `dtype`, dense and 16-byte aligned. residual_out may be residual or x (in place); it is required with residual, and
  * post_weight and gate without residual are refused (DUQ4_ERR_NULL). The products are rounded one by one in the order
- * written, in 32 bits; the sums of squares keep their rounding errors, so results equal those of the steps taken one by
- * one. `format` and the results: DUQ4_MODE_NONE: out = h itself [rows, cols]; DUQ4_MODE_SYM / DUQ4_MODE_ASYM (fp16 only):
+ * written, in 32 bits; the sums of squares keep their rounding errors and the root is taken in 64 bits, so results are those of
+ * the steps taken one by one with means in 64 bits, but where such a root lies within about 1e-15 of the middle of two
+ * floats. `format` and the results: DUQ4_MODE_NONE: out = h itself [rows, cols]; DUQ4_MODE_SYM / DUQ4_MODE_ASYM (fp16 only):
  * out = int4 codes, scales = fp16 [rows], row_scales = fp16 zero-points [rows] (ASYM), as duq4_quantize_{sym,asym}_fused
  * gives them for h; DUQ4_FP4_*: out = codes, scales = block scales, row_scales = float [rows] (NV). cols % 32 == 0, at
  * most 65536. */

@@ -41,3 +41,41 @@ def test_reciprocal_root_next_to_a_border(dtype, rows):
             if not (got == float(want)).all():
                 wrong.append((float(middle), side))
     assert not wrong, (len(wrong), wrong[:4])
+
+
+def _product(silu, up):
+    return (silu.float() * up.float()).to(silu.dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("pin", [16.0, 128.0])
+def test_silu_of_every_gate(dtype, pin):
+    """Each finite gate whose silu is not too small, twice, with the ups between which its product passes 2.5, the border of the
+    codes of 2 and 3 under a scale of 1. The first of each block of 32 pins that scale with a product of 4 (and, by its own gate,
+    which of the two quotients its neighbour takes). A silu that is one unit off would show in most of these codes."""
+    bits = torch.arange(65536, dtype=torch.int32).to(torch.int16).cuda()
+    g = bits.view(dtype)
+    s = torch.nn.functional.silu(g)
+    big = torch.finfo(dtype).max / 2        # ups stay finite; bfloat16's also stay normal
+    keep = g.isfinite() & (s.abs() > 2.5 / big) & (s.abs() < big)
+    g, s = g[keep], s[keep]
+    assert g.numel() > 20000
+    # the first up (by magnitude) whose product is beyond 2.5: from a few units below the quotient upwards
+    near = (2.5 / s.double()).to(dtype).view(torch.int16)
+    ups = torch.stack([(near + d).view(dtype) for d in range(-4, 5)])
+    beyond = _product(s, ups).abs() > 2.5
+    assert beyond[-1].all() and not beyond[0].any()
+    first = beyond.int().argmax(0, keepdim=True)
+    hi, lo = ups.gather(0, first)[0], ups.gather(0, first - 1)[0]
+
+    def blocks(t, pinned):
+        t = torch.cat([t, t[-1:].expand(-t.numel() % (31 * 8))]).view(-1, 31)
+        return torch.cat([torch.full_like(t[:, :1], pinned), t], 1).view(-1, 256)
+    gate, up = blocks(torch.cat([g, g]), pin), blocks(torch.cat([hi, lo]), 4 / pin)
+    silu = blocks(torch.cat([s, s]), pin)
+    want = ops().fp4_quantize("mxfp4", _product(silu, up))[0]
+    assert torch.equal(ops().fp4_silu_mul_quantize("mxfp4", torch.cat([gate, up], 1))[0], want)
+    for d in (-1, 1):   # the cases tell a silu apart that is one unit smaller or larger
+        off = blocks((torch.cat([s, s]).view(torch.int16) + d).view(dtype), pin)
+        other = ops().fp4_quantize("mxfp4", _product(off, up))[0]
+        assert (other != want).sum() > g.numel() // 4
