@@ -121,8 +121,9 @@ __device__ __forceinline__ void issue_stage(uint32_t d, uint64_t da, uint64_t db
     }
 }
 
-// y = acc * token factor * channel factor + bias
-__device__ __forceinline__ float finish(float acc, float ra, float rw, float b) { return __fmaf_rn(__fmul_rn(acc, ra), rw, b); }
+// y = acc * channel factor * token factor + bias. The channel's first: weights are about as large in every layer, while tokens reach
+// over the range of bfloat16, and a sum of up to 2^23 K times the token's factor alone would leave that of 32 bits.
+__device__ __forceinline__ float finish(float acc, float ra, float rw, float b) { return __fmaf_rn(__fmul_rn(acc, rw), ra, b); }
 
 __device__ __forceinline__ uint32_t ctarank() {
     uint32_t r;
