@@ -48,7 +48,6 @@ constexpr int kTileBytes = 512;     // scale tile: 128 rows x 4 blocks
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int code) {
     return mbar_wait(bar, parity, abort_flag, &g_fp4_status, code);
 }
-
 // The wait itself, run out: one warp waits on a barrier that nothing arrives at. `gave_up`: 1 if the first wait reported so, 2 more
 // if the next one, with the CTA aborting, did not wait again.
 __global__ void fp4_wait_selftest_kernel(int *gave_up) {
@@ -798,7 +797,7 @@ static uint32_t pair_columns(uint32_t M, uint32_t N, uint32_t K, uint64_t sms) {
 }
 template <int FMT, class T>
 static int gemm(const GemmArgs &a, cudaStream_t st, uint32_t early) {
-    const uint32_t n0 = pair_columns(a.M, a.N, a.K, (uint64_t)sm_count_current_device());
+    const uint32_t n0 = a.M <= 128 ? 0 : pair_columns(a.M, a.N, a.K, (uint64_t)sm_count_current_device());
     if (n0 == 0) return launch_swap<FMT, T>(a, st, early);
     if (n0 == a.N) return launch_pair<FMT, T>(a, st);
     GemmArgs main = a, left = a;
