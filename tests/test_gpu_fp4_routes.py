@@ -156,3 +156,34 @@ def test_routes_side_by_side(fmt):
                 outs.append((ops().linear_fp4_from_16bit(*args), want))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in outs)
+
+
+def test_beside_the_integer_products():
+    """fp4 and integer products on streams of their own: kernels that take all of TMEM, some of it and clusters that wait for one
+    another meet on the same SMs."""
+    import ctypes
+    import duqlinear4bitcuda_b200.lib as L
+    jobs = []
+    for i, (m, n, k) in enumerate([(64, 22016, 1024), (100, 4096, 4096), (512, 8192, 2048), (48, 9472, 512)]):
+        g = torch.Generator(device="cuda").manual_seed(i)
+        a, w = (torch.randint(0, 256, (r, k // 2), generator=g, device="cuda", dtype=torch.uint8) for r in (m, n))
+        sa, sw = (torch.rand(r, generator=g, device="cuda").half() * 0.01 for r in (m, n))
+        jobs.append((lambda a=a, w=w, sa=sa, sw=sw: ops().linear_w4a4("sym", a, w, sa, None, sw)))
+    for i, (fmt, m, n, k) in enumerate([("nvfp4", 4, 2048, 1024), ("mxfp4", 16, 1024, 2048), ("nvfp4", 40, 4096, 512), ("mxfp4", 128, 4096, 4096),
+                                        ("nvfp4", 300, 3000, 1056), ("mxfp4", 1, 9000, 96)]):
+        x, w, bias = layer(fmt, m, n, k, B, i)
+        jobs.append((lambda fmt=fmt, x=x, w=w, bias=bias: ops().linear_fp4_from_16bit(fmt, x, *w, bias)))
+    want = [j() for j in jobs]
+    streams = [torch.cuda.Stream() for _ in jobs]
+    torch.cuda.synchronize()
+    outs = []
+    for r in range(30):
+        for i in range(len(jobs)):
+            i = (i * 3 + r) % len(jobs)
+            with torch.cuda.stream(streams[i]):
+                outs.append((jobs[i](), want[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in outs)
+    status = ctypes.c_int32(-1)
+    L.call("duq4_last_device_status", L.current_stream(), ctypes.byref(status))
+    assert status.value == 0
