@@ -66,7 +66,8 @@ class NormResidualQuantizer(torch.nn.Module):
 
     norm(t) = t / sqrt(mean(t^2) + eps) over the last dimension. residual: like x. gate: None, [dim], or what broadcasts to x
     (one per sequence, [B, 1, dim], is copied to one per token). format: "mxfp4" / "nvfp4" (a PackedFP4Tensor for
-    LinearFP4), "sym" / "asym" (a PackedQuantizedTensor for the integer layers, fp16), "none" (the norm itself). input_clip_ratio: as SymQuantizer's, for "sym" only. dim % 32 == 0."""
+    LinearFP4), "sym" / "asym" (a PackedQuantizedTensor for the integer layers, fp16), "none" (the norm itself).
+    input_clip_ratio: as SymQuantizer's, for "sym" only. dim % 32 == 0."""
 
     def __init__(self, dim, format="nvfp4", eps=1e-6, post_norm=False, residual_scale=1.0, dtype=torch.float16, input_clip_ratio=1.0):
         super().__init__()

@@ -542,7 +542,7 @@ int duq4_linear_fp4(int format, const uint8_t *A, const uint8_t *A_block_scales,
  * becomes 3 (1: the wait reported that it gave up, 2: the next one did not wait again). Nothing else is touched. */
 int duq4_fp4_wait_selftest(int32_t *result, void *stream);
 /* Which kernels such a product runs on a GPU of `sms` SMs: how many of its N columns the CTA-pair kernel computes. 0: none, all
- * are the few-token kernel's; N: all; between: the rest is a second launch. Host arithmetic only; tests hold their sizes to it. */
+ * are the few-token kernel's; N: all; between: the rest is a second launch. Host arithmetic only. */
 uint32_t duq4_linear_fp4_pair_columns(uint32_t M, uint32_t N, uint32_t K, uint32_t sms);
 /* The same from 16-bit activations x [M, K] (dense): quantized into `workspace` (device memory, 256-byte aligned,
  * duq4_linear_fp4_workspace_bytes bytes), then multiplied. Calls that share a workspace must not overlap on the GPU. */
