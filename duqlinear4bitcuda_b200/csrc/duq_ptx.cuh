@@ -52,9 +52,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
         }
     }
 }
-// A CTA in which a wait ran out lets its copies land before it gives its shared memory back. Called where it
-// does not matter which warp gave up (behind a barrier of the CTA): the one that consumes may, when the producer has long
-// issued its last copy.
+// A CTA in which a wait ran out lets its copies land before it gives its shared memory back. Called by the role that issues
+// copies and by the one that consumes them, where its own wait has failed: the latter may give up when the former has long issued
+// its last copy, and the CTA stays while either holds.
 __device__ __forceinline__ void leave_copies_behind() {
     const uint64_t t0 = globaltimer();
     while (globaltimer() - t0 < 200000ull) __nanosleep(1000);

@@ -312,6 +312,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 if (++s == C::kStages) { s = 0; ph ^= 1; }
             }
         }
+        if (!ok) leave_copies_behind();
     } else if (warp == 1) {
         if (rank == 0) {
             uint32_t s = 0, ph = 0, lt = 0;
@@ -351,6 +352,7 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
                 const uint64_t t0 = globaltimer();
                 while (!mbar_try(drained, 0) && globaltimer() - t0 < kPtxWaitLimitNs) __nanosleep(1000);
             }
+            if (!ok) leave_copies_behind();   // both producers may have issued their last copies long ago; the pair ends together
         }
     } else {
         // Epilogue, eight warps: two per TMEM lane quadrant, which take the tile's 32-column chunks in turn, the shared
@@ -400,8 +402,6 @@ fp4_pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
-    if (abort_flag && warp == 0) leave_copies_behind();   // whichever wait ran out; before the partner's memory may go
-    __syncwarp();
     cluster_barrier();   // the partner is done with this CTA's shared memory and TMEM
     if (warp == 1) {
         __syncwarp();
@@ -513,6 +513,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
     };
     if (warp == 0) {
+        bool ok = true;
         if (p.early == 1) {
             asm volatile("griddepcontrol.wait;" ::: "memory");
             for (uint32_t i = 0; i < head; ++i) {
@@ -522,7 +523,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
         }
         uint32_t s = 0, ph = 1;
         for (uint32_t i = head; i < k1 - k0; ++i) {
-            if (!wait(empty(s), ph ^ 1, abortp, 11)) break;
+            if (!(ok = wait(empty(s), ph ^ 1, abortp, 11))) break;
             if (elected()) {
                 weights(k0 + i, s);
                 tokens(k0 + i, s);
@@ -530,6 +531,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             __syncwarp();
             if (++s == p.stages) { s = 0; ph ^= 1; }
         }
+        if (!ok) leave_copies_behind();
     } else if (warp == 1) {
         if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");   // the launch in front may take longer than a wait on a barrier may
         bool ok = true, issued = false;
@@ -554,6 +556,7 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             const uint64_t b0 = globaltimer();
             while (!mbar_try(drained, 0) && globaltimer() - b0 < kPtxWaitLimitNs) __nanosleep(1000);
         }
+        if (!ok) leave_copies_behind();   // the producer may have issued its last copy long ago
     } else {
         terms();
         if (p.early == 1) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -634,7 +637,6 @@ fp4_swap_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant
             gather(integral_constant<int, 1>{}, integral_constant<int, 8>{});
         }
     }
-    if (abort_flag && warp == 0) leave_copies_behind();   // whichever wait ran out: copies may be under way although every load was issued
     __syncwarp();
     if (p.splits > 1) cluster_barrier();   // the others have read this CTA's partial sums
     if (p.early == 2) asm volatile("griddepcontrol.wait;" ::: "memory");   // this launch does not end before the one in front
