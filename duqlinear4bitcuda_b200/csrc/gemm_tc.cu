@@ -162,6 +162,7 @@ __global__ void __launch_bounds__(threads_for(UW), 1) gemm_tc_kernel(const __gri
                     }
                 }
             }
+            if (!ok) leave_copies_behind();
         }
     } else if (MODE == MODE_A8B4 && warp == kLastWarp) {
         // ---------------- second TMA producer: pre-unpacked A straight into the MMA ring ----------------
@@ -179,6 +180,7 @@ __global__ void __launch_bounds__(threads_for(UW), 1) gemm_tc_kernel(const __gri
                     tma_load_3d(up0 + u * C::kUnpackedStage, &tmA, up_full(u), ks * BK, tm * BM, b);
                 }
             }
+            if (!ok) leave_copies_behind();
         }
     } else if (warp == 1) {
         // ---------------- MMA issuer ----------------
@@ -210,6 +212,7 @@ __global__ void __launch_bounds__(threads_for(UW), 1) gemm_tc_kernel(const __gri
                 uint64_t t0 = globaltimer();
                 while (!mbar_try(drain_bar, 0) && globaltimer() - t0 < kWaitLimitNs) __nanosleep(1000);
             }
+            if (!ok) leave_copies_behind();   // the producers may have issued their last copies long ago
         }
     } else if (warp < 2 + kEpiWarps) {
         // ---------------- epilogue ----------------
@@ -273,11 +276,11 @@ __global__ void __launch_bounds__(threads_for(UW), 1) gemm_tc_kernel(const __gri
                 }
             }
         }
+        if (!ok) leave_copies_behind();
     }
 
     tc_fence_before();
     __syncthreads();
-    if (abort_flag && warp == 0) leave_copies_behind();
     if (warp == 1) {
         __syncwarp();
         tc_fence_after();
